@@ -58,6 +58,13 @@ extern "C" {
 #define MFL_OP_MEANFIELD_FORWARD 3
 #define MFL_OP_MEANFIELD_BACKWARD 4
 
+/* element types of the score tensors of mfl_top_labels, mfl_distillation_* and mfl_sample_labels */
+#define MFL_F32 0
+#define MFL_BF16 1
+#define MFL_F16 2
+/* most labels a record of top labels holds */
+#define MFL_MAX_TOP_LABELS 128
+
 typedef void *mfl_stream_t;
 
 /* Library version (MFL_VERSION of the build). */
@@ -332,6 +339,69 @@ int mfl_preprocess_rgb8(const unsigned char *src, int H0, int W0, const int *xco
  */
 int mfl_resize_labels(const unsigned char *src, int H0, int W0, const int *yin, const int *xin, unsigned char *out, int H,
                       int W, mfl_stream_t stream);
+
+/*
+ * Operators on rows of scores.  A row is one distribution over C labels; element (n, c, s) of N x C x S scores lies at
+ * scores + n * stride_n + c * stride_c + s * stride_s (elements; not negative), so [B][C][H][W] maps (S = H*W), [N][C]
+ * matrices (S = 1), channels-last maps and slices are read where they are.  dtype: MFL_F32, MFL_BF16 or MFL_F16.
+ * N * S < 2^31 and C <= 2^30 (MFL_ERR_TOO_LARGE); offsets are 64-bit.  b = score / temperature throughout.
+ * Results do not depend on the launch or on timing: no floating-point atomics.
+ *
+ * mfl_top_labels: the k largest scores of every row, descending, the lower label first among equals (a NaN counts as
+ * larger than any number), and rest = log sum exp(b) over the other labels (-inf if there are none): what a teacher
+ * keeps for mfl_distillation_*.  k = 1 answers like mfl_argmax_labels.  The reference has no counterpart.
+ *   values: [N][k][S] of the scores' type   labels: [N][k][S] int32   rest: [N][S] float
+ *   1 <= k <= min(C, MFL_MAX_TOP_LABELS), 1e-30 <= temperature <= 1e30
+ */
+size_t mfl_top_labels_workspace_bytes(int N, int C, int S, int dtype, int k);
+int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c,
+                   long long stride_s, double temperature, int k, void *values, int *labels, float *rest,
+                   void *workspace, size_t workspace_bytes, mfl_stream_t stream);
+
+/*
+ * Distillation loss of every row against a teacher's record, and its gradient (the reference trains on one label per
+ * pixel with the NLL of AdvancedModel.py:295-299; this is the same step against a distribution):
+ *   p = the teacher's shares: its k entries and, with `rest`, everything else as one more outcome
+ *   q = softmax(b), q_rest = its mass outside the record
+ *   loss = T^2 ( sum_j p_j log(p_j / q_j) + p_rest log(p_rest / q_rest) )
+ * Entries with a label outside [0, C) belong to no class and are passed over (a record padded with -1); an entry named
+ * twice counts as two entries.  Rows with valid = 0, without any teacher mass or whose scores are all -inf have loss 0
+ * and gradient 0, whatever the other tensors hold there.
+ *   values: [N][k][S] of values_dtype   labels: [N][k][S] int32   rest: [N][S] float or NULL (entries renormalised)
+ *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [4][N][S] floats, from forward to backward
+ *   grad_loss: [N][S]   d_scores: the scores' type, with strides of its own, overwritten
+ */
+size_t mfl_distillation_workspace_bytes(int N, int C, int S, int dtype, int k);
+int mfl_distillation_forward(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c,
+                             long long stride_s, const void *values, int values_dtype, const int *labels,
+                             const float *rest, const unsigned char *valid, int k, double temperature, float *loss,
+                             float *stats, void *workspace, size_t workspace_bytes, mfl_stream_t stream);
+int mfl_distillation_backward(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c,
+                              long long stride_s, const void *values, int values_dtype, const int *labels,
+                              const float *rest, const unsigned char *valid, int k, double temperature,
+                              const float *stats, const float *grad_loss, void *d_scores, long long d_stride_n,
+                              long long d_stride_c, long long d_stride_s, mfl_stream_t stream);
+
+/*
+ * One label per row drawn from the given random numbers (mfl_argmax_labels answers with the largest marginal, this
+ * follows the marginals).  With w = exp((score - largest) / T) and the labels ranked as in mfl_top_labels: keep the
+ * first top_k; of those the ones in front of which less than top_p of their mass lies; of those the ones with
+ * w >= min_p (the first always stays).  labels = the first kept label, in label order, whose running sum exceeds
+ * uniform * (kept mass); logprob = log of its share of that mass.  Sums are 64-bit.
+ *   uniform: [N][S] in [0, 1) (below: 0; 1 and above: the last kept label)
+ *   temperature (0: the largest score), top_k (0: all), top_p in (0, 1], min_p in [0, 1]: each for all rows, or, where
+ *   the array next to it is not NULL, [N] values of which temperature <= 0, top_k <= 0, top_p >= 1, min_p <= 0 mean the
+ *   same as 0, 0, 1, 0
+ *   labels: [N][S] of label_bytes 1 (C <= 255), 4 or 8   logprob: [N][S] or NULL
+ * A row without a finite largest score (all -inf, or a NaN or +inf among them): label -1 (255 in one byte, the void
+ * label), logprob -inf.
+ */
+size_t mfl_sample_labels_workspace_bytes(int N, int C, int S, int dtype);
+int mfl_sample_labels(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c,
+                      long long stride_s, const float *uniform, double temperature, const float *temperature_n,
+                      int top_k, const int *top_k_n, double top_p, const float *top_p_n, double min_p,
+                      const float *min_p_n, void *labels, int label_bytes, float *logprob, void *workspace,
+                      size_t workspace_bytes, mfl_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,6 +21,10 @@ OP_MEANFIELD_FORWARD = 3
 OP_MEANFIELD_BACKWARD = 4
 
 _c_int, _c_size, _c_void = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
+_c_ll, _c_double = ctypes.c_longlong, ctypes.c_double
+_SCORES = [_c_void] + [_c_int] * 4 + [_c_ll] * 3        # scores, dtype, N, C, S and three strides
+SCORE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # MFL_F32, MFL_BF16, MFL_F16
+MAX_TOP_LABELS = 128
 
 # name -> (restype, argtypes); mirrors include/mfl.h one to one
 SIGNATURES = {
@@ -47,6 +51,16 @@ SIGNATURES = {
                                      _c_void, _c_size, _c_void]),
     "mfl_resize_labels": (_c_int, [_c_void, _c_int, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int, _c_void]),
     "mfl_iou_counts": (_c_int, [_c_void, _c_void, _c_void, _c_size, _c_int, _c_void]),
+    "mfl_top_labels_workspace_bytes": (_c_size, [_c_int] * 5),
+    "mfl_top_labels": (_c_int, _SCORES + [_c_double, _c_int] + [_c_void] * 4 + [_c_size, _c_void]),
+    "mfl_distillation_workspace_bytes": (_c_size, [_c_int] * 5),
+    "mfl_distillation_forward": (_c_int, _SCORES + [_c_void, _c_int] + [_c_void] * 3 + [_c_int, _c_double] + [_c_void] * 3
+                                 + [_c_size, _c_void]),
+    "mfl_distillation_backward": (_c_int, _SCORES + [_c_void, _c_int] + [_c_void] * 3 + [_c_int, _c_double] + [_c_void] * 3
+                                  + [_c_ll] * 3 + [_c_void]),
+    "mfl_sample_labels_workspace_bytes": (_c_size, [_c_int] * 4),
+    "mfl_sample_labels": (_c_int, _SCORES + [_c_void, _c_double, _c_void, _c_int, _c_void, _c_double, _c_void, _c_double, _c_void,
+                                             _c_void, _c_int, _c_void, _c_void, _c_size, _c_void]),
     "mfl_argmax_labels": (_c_int, [_c_void, _c_void] + [_c_int] * 4 + [_c_void]),
 }
 
@@ -101,6 +115,23 @@ def require_device(*tensors: torch.Tensor) -> None:
                                f"'{t.device}' (there is no CPU fallback)")
         if t.dtype != torch.float32:
             raise RuntimeError(f"expected float32 tensors, got {t.dtype}")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
+
+
+def require_scores(*tensors) -> None:
+    """Score tensors: on one ROCm GPU, float32, bfloat16 or float16 (each its own)."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("semantic_segmentation_amd runs on a ROCm GPU only: got a tensor on "
+                               f"'{t.device}' (there is no CPU fallback)")
+        if t.dtype not in SCORE_DTYPES:
+            raise RuntimeError(f"expected float32, bfloat16 or float16 scores, got {t.dtype}")
         if dev is None:
             dev = t.device
         elif t.device != dev:

@@ -167,6 +167,149 @@ def argmax_labels(logq: torch.Tensor) -> torch.Tensor:
     return labels
 
 
+def _score_rows(t: torch.Tensor, name: str = "scores"):
+    """[N, C] or [N, C, ...] scores as the library reads them: (tensor to keep alive, dtype code, N, C, S, three strides).
+    Nothing is copied where the dimensions behind C have one common stride (contiguous and channels-last maps, slices)."""
+    if t.dim() < 2:
+        raise RuntimeError(f"{name} must be [N, C] or [N, C, ...], got {tuple(t.shape)}")
+    if t.numel() == 0:
+        raise RuntimeError(f"{name} is empty: {tuple(t.shape)}")
+    v = t.detach()
+    v = v.unsqueeze(2) if v.dim() == 2 else v.flatten(2)
+    return v, (_lib.SCORE_DTYPES[t.dtype],) + tuple(v.shape) + tuple(v.stride())
+
+
+def _like_rows(t: torch.Tensor, x, name: str, dtypes, shape):
+    """A tensor beside the scores: its device, type and shape checked, contiguous."""
+    if not x.is_cuda or x.device != t.device:
+        raise RuntimeError(f"{name} must be on {t.device}, got {x.device}")
+    if x.dtype not in dtypes:
+        raise RuntimeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {x.dtype}")
+    if tuple(x.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must be {tuple(shape)}, got {tuple(x.shape)}")
+    return x.detach().contiguous()
+
+
+def _score_workspace(n: int, t: torch.Tensor):
+    return torch.empty(n, dtype=torch.uint8, device=t.device) if n else None
+
+
+def top_labels(scores: torch.Tensor, k: int, temperature: float = 1.0):
+    """The k largest scores of every row of [N, C] or [N, C, ...] scores, descending, the lower label first among equals:
+    (values [N, k, ...] of the scores' type, labels [N, k, ...] int32, rest [N, ...] float32), with rest = log sum
+    exp(score / temperature) over all other labels (-inf if there are none).  The record distillation_forward reads."""
+    _lib.require_scores(scores)
+    v, args = _score_rows(scores)
+    if not 1 <= k <= min(args[2], _lib.MAX_TOP_LABELS):
+        raise ValueError(f"k must be between 1 and min(C, {_lib.MAX_TOP_LABELS}), got {k} with C = {args[2]}")
+    shape = tuple(scores.shape)
+    values = torch.empty((shape[0], k) + shape[2:], dtype=scores.dtype, device=scores.device)
+    labels = torch.empty((shape[0], k) + shape[2:], dtype=torch.int32, device=scores.device)
+    rest = torch.empty((shape[0],) + shape[2:], dtype=torch.float32, device=scores.device)
+    with torch.cuda.device(scores.device):
+        n = int(lib.mfl_top_labels_workspace_bytes(args[1], args[2], args[3], args[0], k))
+        ws = _score_workspace(n, scores)
+        _lib.check(lib.mfl_top_labels(ptr(v), *args, float(temperature), k, ptr(values), ptr(labels), ptr(rest), ptr(ws), n,
+                                      stream_of(scores)), "mfl_top_labels")
+    return values, labels, rest
+
+
+def _record(scores, top_scores, top_labels, rest, valid):
+    """The teacher's side of a distillation call, checked: (values, labels, rest, valid as bytes)."""
+    shape = tuple(scores.shape)
+    if top_scores.dim() != scores.dim():
+        raise RuntimeError(f"top_scores must be [N, k, ...] beside scores {shape}, got {tuple(top_scores.shape)}")
+    k = top_scores.shape[1]
+    if not 1 <= k <= _lib.MAX_TOP_LABELS:
+        raise ValueError(f"a record holds between 1 and {_lib.MAX_TOP_LABELS} labels, got {k}")
+    rows, record = (shape[0],) + shape[2:], (shape[0], k) + shape[2:]
+    top_scores = _like_rows(scores, top_scores, "top_scores", tuple(_lib.SCORE_DTYPES), record)
+    top_labels = _like_rows(scores, top_labels, "top_labels", (torch.int32,), record)
+    rest = None if rest is None else _like_rows(scores, rest, "rest", (torch.float32,), rows)
+    valid = None if valid is None else _like_rows(scores, valid, "valid", (torch.bool, torch.uint8), rows)
+    return top_scores, top_labels, rest, valid
+
+
+def distillation_forward(scores, top_scores, top_labels, rest=None, temperature: float = 1.0, valid=None):
+    """Loss of every row of [N, C, ...] scores against a teacher's record (top_labels of the teacher's scores at the same
+    temperature): T^2 KL(teacher || softmax(scores / T)) over the record's labels and, with `rest`, everything else as one
+    more outcome; without it the record is renormalised.  Labels outside [0, C) are passed over; rows with valid = False or
+    without teacher mass have loss 0.  Returns (loss [N, ...] float32, stats for distillation_backward)."""
+    _lib.require_scores(scores)
+    v, args = _score_rows(scores)
+    values, labels, rest, valid = _record(scores, top_scores, top_labels, rest, valid)
+    rows = (scores.shape[0],) + tuple(scores.shape[2:])
+    loss = torch.empty(rows, dtype=torch.float32, device=scores.device)
+    stats = torch.empty((4,) + rows, dtype=torch.float32, device=scores.device)
+    k = values.shape[1]
+    with torch.cuda.device(scores.device):
+        n = int(lib.mfl_distillation_workspace_bytes(args[1], args[2], args[3], args[0], k))
+        ws = _score_workspace(n, scores)
+        _lib.check(lib.mfl_distillation_forward(ptr(v), *args, ptr(values), _lib.SCORE_DTYPES[values.dtype], ptr(labels), ptr(rest),
+                                                ptr(valid), k, float(temperature), ptr(loss), ptr(stats), ptr(ws), n,
+                                                stream_of(scores)), "mfl_distillation_forward")
+    return loss, stats
+
+
+def distillation_backward(scores, top_scores, top_labels, stats, grad_loss, rest=None, temperature: float = 1.0, valid=None):
+    """Gradient of sum(grad_loss * loss) of distillation_forward with respect to the scores, in their type and layout;
+    the other arguments as there, stats as it returned them."""
+    _lib.require_scores(scores)
+    v, args = _score_rows(scores)
+    values, labels, rest, valid = _record(scores, top_scores, top_labels, rest, valid)
+    rows = (scores.shape[0],) + tuple(scores.shape[2:])
+    stats = _like_rows(scores, stats, "stats", (torch.float32,), (4,) + rows)
+    grad_loss = _like_rows(scores, grad_loss, "grad_loss", (torch.float32,), rows)
+    grad = torch.empty_like(scores, requires_grad=False)
+    g, gargs = _score_rows(grad, "gradient")
+    if g.data_ptr() != grad.data_ptr():                  # (a layout without one common stride)
+        grad = torch.empty_like(scores, memory_format=torch.contiguous_format, requires_grad=False)
+        g, gargs = _score_rows(grad, "gradient")
+    with torch.cuda.device(scores.device):
+        _lib.check(lib.mfl_distillation_backward(ptr(v), *args, ptr(values), _lib.SCORE_DTYPES[values.dtype], ptr(labels), ptr(rest),
+                                                 ptr(valid), values.shape[1], float(temperature), ptr(stats), ptr(grad_loss), ptr(g),
+                                                 *gargs[4:], stream_of(scores)), "mfl_distillation_backward")
+    return grad
+
+
+_SAMPLE_LABEL_TYPES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
+
+
+def sample_labels(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, dtype=torch.int64, want_logprob: bool = False):
+    """One label per row of [N, C] or [N, C, ...] scores, drawn with the given random numbers uniform [N, ...] in [0, 1):
+    argmax_labels' counterpart that follows the distribution softmax(scores / temperature), cut to the top_k largest (0:
+    all), then to the shortest descending run with top_p of their mass, then to what has min_p of the largest's share.
+    The label is the first kept one, in label order, whose running sum exceeds uniform * (kept mass).  temperature 0 takes
+    the largest.  Each setting is a number or a tensor of N values (float32; top_k int32), in which temperature <= 0,
+    top_k <= 0, top_p >= 1 and min_p <= 0 mean the same as 0, 0, 1 and 0.  A row without a finite largest score (all -inf,
+    or a NaN or +inf in it) gets label -1 (255, the void label, with dtype=torch.uint8, which needs C <= 255).
+    Returns labels [N, ...], or (labels, logprob) with the logarithm of the drawn label's share of the kept mass."""
+    _lib.require_scores(scores)
+    v, args = _score_rows(scores)
+    N, rows = scores.shape[0], (scores.shape[0],) + tuple(scores.shape[2:])
+    uniform = _like_rows(scores, uniform, "uniform", (torch.float32,), rows)
+    if dtype not in _SAMPLE_LABEL_TYPES:
+        raise TypeError(f"labels are uint8, int32 or int64, not {dtype}")
+    if dtype == torch.uint8 and args[2] > 255:
+        raise ValueError(f"uint8 labels hold at most 255 labels and the void one, got C = {args[2]}")
+    settings = []
+    for name, x, kind in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                          ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(x):
+            settings += [0 if kind == torch.int32 else 0.0, _like_rows(scores, x, name, (kind,), (N,))]
+        else:
+            settings += [int(x) if kind == torch.int32 else float(x), None]
+    labels = torch.empty(rows, dtype=dtype, device=scores.device)
+    logprob = torch.empty(rows, dtype=torch.float32, device=scores.device) if want_logprob else None
+    with torch.cuda.device(scores.device):
+        n = int(lib.mfl_sample_labels_workspace_bytes(args[1], args[2], args[3], args[0]))
+        ws = _score_workspace(n, scores)
+        call = [ptr(x) if torch.is_tensor(x) or x is None else x for x in settings]
+        _lib.check(lib.mfl_sample_labels(ptr(v), *args, ptr(uniform), *call, ptr(labels), _SAMPLE_LABEL_TYPES[dtype], ptr(logprob),
+                                         ptr(ws), n, stream_of(scores)), "mfl_sample_labels")
+    return (labels, logprob) if want_logprob else labels
+
+
 def label_context_forward(t, conv_w, unary, conv_b=None, la_w=None, la_b=None, ga_w=None, ga_b=None, mixtures=None,
                           want_smooth=False, keep=False):
     """DPNModel.forward phases 3-4 behind the local convolution (AdvancedModel.py:223, 232-244): per-pixel affine,

@@ -13,7 +13,9 @@ from typing import Callable, Iterable, Optional, Tuple
 import torch
 from torch import nn
 
-from . import parallel
+from torch.autograd.function import once_differentiable
+
+from . import ops, parallel
 
 
 def class_weights(labels: torch.Tensor, num_labels: int) -> torch.Tensor:
@@ -38,6 +40,47 @@ def per_image_nll(log_probs: torch.Tensor, labels: torch.Tensor, weight: Optiona
         denom = (weight[labels.clamp(max=weight.numel() - 1)] * valid).flatten(1).sum(1)
     per_image = losses.flatten(1).sum(1) / denom.clamp(min=torch.finfo(losses.dtype).tiny)
     return torch.where(denom > 0, per_image, torch.zeros_like(per_image)).mean()
+
+
+class _DistillationFunction(torch.autograd.Function):
+    """Per-row distillation loss; backward by the library."""
+
+    @staticmethod
+    def forward(ctx, scores, top_scores, top_labels, rest, temperature, valid):
+        loss, stats = ops.distillation_forward(scores, top_scores, top_labels, rest, temperature, valid)
+        ctx.temperature = temperature
+        ctx.save_for_backward(scores, top_scores, top_labels, rest, valid, stats)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        scores, top_scores, top_labels, rest, valid, stats = ctx.saved_tensors
+        grad = ops.distillation_backward(scores, top_scores, top_labels, stats, grad_loss, rest, ctx.temperature, valid)
+        return grad, None, None, None, None, None
+
+
+def distillation_loss(scores: torch.Tensor, top_scores: torch.Tensor, top_labels: torch.Tensor,
+                      rest: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                      valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Loss of every row of [N, C] or [N, C, ...] scores (or log-marginals) against a teacher's record, as
+    ops.distillation_forward defines it, with its gradient: the counterpart of an NLL without reduction whose target is
+    the teacher's distribution.  The record (ops.top_labels of the teacher's scores at the same temperature) has no
+    gradient."""
+    if top_scores.requires_grad or (rest is not None and rest.requires_grad):
+        raise RuntimeError("distillation_loss: no gradient for the teacher's record; detach it")
+    return _DistillationFunction.apply(scores, top_scores, top_labels, rest, temperature, valid)
+
+
+def per_image_distillation(scores: torch.Tensor, top_scores: torch.Tensor, top_labels: torch.Tensor,
+                           rest: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                           valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Mean over the batch of every image's mean distillation loss over its valid pixels: per_image_nll with the teacher's
+    distribution as the target.  An image without a valid pixel contributes 0."""
+    losses = distillation_loss(scores, top_scores, top_labels, rest, temperature, valid).flatten(1)
+    if valid is None:
+        return losses.mean(1).mean()
+    return (losses.sum(1) / (valid != 0).flatten(1).sum(1).clamp(min=1)).mean()
 
 
 def fit(model: nn.Module, optimizer: torch.optim.Optimizer,
