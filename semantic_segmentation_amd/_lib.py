@@ -121,21 +121,17 @@ def require_device(*tensors: torch.Tensor) -> None:
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
 
 
-def require_scores(*tensors) -> None:
-    """Score tensors: on one ROCm GPU, float32, bfloat16 or float16 (each its own)."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("semantic_segmentation_amd runs on a ROCm GPU only: got a tensor on "
-                               f"'{t.device}' (there is no CPU fallback)")
-        if t.dtype not in SCORE_DTYPES:
-            raise RuntimeError(f"expected float32, bfloat16 or float16 scores, got {t.dtype}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
+def call_scores(fn, what: str, t: torch.Tensor, *args) -> None:
+    """One call on rows of scores, queued on the current stream of the scores' device (small calls are bound by the
+    host: no device switch where the device is current, the stream as a plain number)."""
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        check(code, what)
 
 
 _PLANS = {}          # (op, B, C, H, W, k, iters, device) -> workspace kept between calls (keep_plans(True))

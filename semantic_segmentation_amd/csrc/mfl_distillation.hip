@@ -33,39 +33,28 @@ struct Teacher {
 };
 
 constexpr int kLaneThreads = 256;
-constexpr int kChunkWords = 8;          // labels marked at a time by a lane: 32 * 8 bits
 
-// The teacher's side of one row, by one lane: running sum over the entries (units of scores) and the rest.
+// The teacher's distribution of a row.  log p_j = (t_j - m) / T - l, log p_rest = rest - m / T - l
 struct Target {
-    LogSum sum;
-    float log_a;                // A - sum.m / T
-    float log_p_rest, p_rest;
-    bool any;                   // the teacher's distribution holds something
+    float m, l, log_p_rest, p_rest;
+    bool any;                   // it holds something
 };
-__device__ inline Target target_of(const Teacher &t, int C, size_t base, size_t step, unsigned r)
+// sum: the entries with a label of the row (named: there are some); rest: -inf for none
+__device__ inline Target target_of(const Teacher &t, Excess sum, bool named, float rest)
 {
     Target g;
-    g.sum = {-INFINITY, 0.f};
-    g.any = false;
-    for (int j = 0; j < t.k; ++j) {
-        const int i = t.labels[base + j * step];
-        if ((unsigned)i >= (unsigned)C) continue;
-        g.any = true;
-        add_score(g.sum, load_any(t.values, t.dtype, base + j * step), t.c2);
-    }
-    const float rest = t.rest ? t.rest[r] : -INFINITY;
-    // the rest joins in units of the scores: exp(rest) = exp((rest * T) / T)
-    if (rest != -INFINITY) {
-        const float m = fmaxf(g.sum.m, rest * t.t), ref = finite_or_zero(m);
-        g.sum.s = g.sum.s * __builtin_amdgcn_exp2f((g.sum.m - ref) * t.c2) + __builtin_amdgcn_exp2f((rest - ref * t.inv_t) * kLog2e);
-        g.sum.m = m;
-    }
-    g.any = g.any && !(g.sum.s == 0.f);
-    g.log_a = logf(g.sum.s);
-    g.log_p_rest = rest == -INFINITY ? -INFINITY : (rest - g.sum.m * t.inv_t) - g.log_a;
+    if (sum.m == -INFINITY && rest != -INFINITY) sum.m = rest * t.t;
+    const float above = fmaf(-sum.m, t.inv_t, rest);       // the rest next to the largest entry
+    if (rest == -INFINITY) g.l = log_1p(sum.s);
+    else if (above <= 0) g.l = log_1p(sum.s + __builtin_amdgcn_exp2f(above * kLog2e));
+    else g.l = above + log_1p((1.f + sum.s) * __builtin_amdgcn_exp2f(-above * kLog2e));
+    g.m = sum.m;
+    g.any = named && !(sum.m == -INFINITY && sum.s == -1.f);
+    g.log_p_rest = rest == -INFINITY ? -INFINITY : above - g.l;
     g.p_rest = __builtin_amdgcn_exp2f(g.log_p_rest * kLog2e);
     return g;
 }
+__device__ inline float log_share(const Teacher &t, const Target &g, float value) { return (value - g.m) * t.inv_t - g.l; }
 
 // p (log p - log q); nothing where p is 0
 __device__ inline float share_term(float p, float log_p, float log_q) { return p == 0.f ? 0.f : p * (log_p - log_q); }
@@ -74,11 +63,13 @@ struct Stats {
     float m, z, mo, zo;         // as above
 };
 constexpr Stats kNoStats = {-INFINITY, 0.f, -INFINITY, 0.f};
-__device__ inline Stats stats_of(LogSum all, LogSum out, bool rest)
+// top: the record's labels, each once; out: all others
+__device__ inline Stats stats_of(Excess top, LogSum out, float c2)
 {
-    if (all.m == -INFINITY && all.s == 0.f) return kNoStats;
-    const bool some = rest && !(out.m == -INFINITY && out.s == 0.f);
-    return {all.m, logf(all.s), some ? out.m : -INFINITY, some ? logf(out.s) : 0.f};
+    const Excess all = join(top, Excess{out.m, out.s - 1.f}, c2);
+    if (all.m == -INFINITY && all.s == -1.f) return kNoStats;
+    const bool some = !(out.m == -INFINITY && out.s == 0.f);
+    return {all.m, log_1p(all.s), some ? out.m : -INFINITY, some ? logf(out.s) : 0.f};
 }
 __device__ inline float log_q_rest(const Stats &a, float inv_t)
 {
@@ -87,6 +78,7 @@ __device__ inline float log_q_rest(const Stats &a, float inv_t)
 __device__ inline void put(float *loss, float *stats, size_t rows, unsigned r, float l, const Stats &a)
 {
     loss[r] = l;
+    if (!stats) return;
     stats[r] = a.m;
     stats[rows + r] = a.z;
     stats[2 * rows + r] = a.mo;
@@ -125,251 +117,555 @@ __device__ inline float slope(const Slope &s, float x, float taken, float c2)
     return named ? s.up * (e - taken) : s.f_out * e;
 }
 
-// One lane per row: see mfl_top_labels.hip for the shapes of work.
-template <typename T, bool REST>
+// ---- one lane per row (see mfl_top_labels.hip for the two shapes of work)
+//
+// A lane takes its labels CB at a time and its record's entries KB at a time, all loads of a block in flight at once; the
+// student's scores of the record are fetched by label beside the stream.  With KB >= k the record stays in registers, with
+// CB >= C the scores do, and the backward pass then finds the softmax statistics by itself instead of reading them back
+// (16 bytes of 200 a pixel at 21 labels).
+
+constexpr int kLoneBlock = 24;          // up to this many labels a lane's scores stay in registers
+
+// Entries j0 .. j0 + KB of a row's record; x: the student's scores of their labels
+template <typename T, int KB> struct Block {
+    int label[KB];              // -1: none, or no label of the row
+    float value[KB], x[KB];
+    __device__ Block(const Rows &in, const Teacher &t, size_t base, int j0)
+    {
+        auto at = [&](int j) { return base + (size_t)min(j0 + j, t.k - 1) * in.S; };
+#pragma unroll
+        for (int j = 0; j < KB; ++j) label[j] = t.labels[at(j)];
+        load_any(value, t.values, t.dtype, at);
+    }
+    __device__ void fetch(const Rows &in, const Teacher &t, const T *p, int j0)
+    {
+        T raw[KB];
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+            label[j] = j0 + j < t.k && (unsigned)label[j] < (unsigned)in.C ? label[j] : -1;
+            raw[j] = p[max(label[j], 0) * in.sc];
+        }
+#pragma unroll
+        for (int j = 0; j < KB; ++j) x[j] = to_float(raw[j]);
+    }
+};
+
+// valid and rest of a row, read from some address without a branch, so that nothing waits for them before they are used
+struct RowFlags {
+    unsigned char v;
+    float r;
+    __device__ RowFlags(const Teacher &t, unsigned row)
+        : v(*(t.valid ? t.valid + row : (const unsigned char *)t.labels)), r(*(t.rest ? t.rest + row : (const float *)t.labels)) {}
+    __device__ bool valid(const Teacher &t) const { return !t.valid || v; }
+    __device__ float rest(const Teacher &t) const { return t.rest ? r : -INFINITY; }
+};
+
+// A record as one lane goes over it: f(block) for all of it, from registers where it fits
+template <typename T, int KB, bool ALL> struct LaneRecord {
+    const Rows &in;
+    const Teacher &t;
+    const T *p;
+    size_t base;
+    Block<T, KB> first;
+    __device__ LaneRecord(const Rows &in, const Teacher &t, const T *p, size_t base) : in(in), t(t), p(p), base(base), first(in, t, base, 0) {}
+    __device__ void fetch() { first.fetch(in, t, p, 0); }
+    template <typename F> __device__ void each(F f) const
+    {
+        f(first);
+        if constexpr (!ALL)
+            for (int j0 = KB; j0 < t.k; j0 += KB) {
+                Block<T, KB> b(in, t, base, j0);
+                b.fetch(in, t, p, j0);
+                f(b);
+            }
+    }
+    __device__ Target target(float rest) const
+    {
+        Excess sum = kNoExcess;
+        bool named = false;
+        each([&](const Block<T, KB> &b) {
+#pragma unroll
+            for (int j = 0; j < KB; ++j) {
+                named |= b.label[j] >= 0;
+                sum = join(sum, b.label[j] >= 0 ? Excess{b.value[j], 0.f} : kNoExcess, t.c2);
+            }
+        });
+        return target_of(t, sum, named, rest);
+    }
+};
+
+// Labels c0 .. c0 + CB of a row (what lies behind the last one: -inf)
+template <typename T, int CB> __device__ inline void load_labels(float (&x)[CB], const Rows &in, const T *p, int c0)
+{
+    T raw[CB];
+    const T *q = p + c0 * in.sc;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        raw[i] = *q;
+        q += c0 + i + 1 < in.C ? in.sc : 0;         // (the last one again)
+    }
+#pragma unroll
+    for (int i = 0; i < CB; ++i) x[i] = i == 0 || c0 + i < in.C ? to_float(raw[i]) : -INFINITY;
+}
+
+// Adds a block of labels to the two sums: the record's into top (each once), the others into out
+template <typename T, int CB, int KB, bool ALL>
+__device__ inline void add_labels(const LaneRecord<T, KB, ALL> &record, const float (&x)[CB], int c0, float c2, LogSum &out, Excess &top)
+{
+    static_assert(CB <= 32, "one word of marks");
+    uint32_t marks = 0;
+    record.each([&](const Block<T, KB> &b) {
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+            const int i = b.label[j] - c0;
+            const bool here = b.label[j] >= 0 && (unsigned)i < (unsigned)CB;
+            const uint32_t bit = here ? 1u << i : 0u;
+            top = join(top, here && !(marks & bit) ? Excess{b.x[j], 0.f} : kNoExcess, c2);
+            marks |= bit;
+        }
+    });
+    float m = out.m, y[CB];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        // (-inf where marked, by its bits: two instructions)
+        const int mark = (int)(marks << (31 - i)) >> 31, bits = __builtin_bit_cast(int, x[i]);
+        y[i] = __builtin_bit_cast(float, (mark & (int)0xff800000) | (~mark & bits));
+        m = fmaxf(m, y[i]);
+    }
+    const float ref = finite_or_zero(m);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) sum += __builtin_amdgcn_exp2f((y[i] - ref) * c2);
+    out = {m, fmaf(out.s, __builtin_amdgcn_exp2f((out.m - ref) * c2), sum)};
+}
+
+// LONE: C <= CB
+template <typename T, int CB, bool LONE, int KB, bool ALL>
 __global__ void __launch_bounds__(kLaneThreads)
 forward_lanes_kernel(Rows in, Teacher t, float *__restrict__ loss, float *__restrict__ stats)
 {
-    __shared__ uint32_t marks[kChunkWords][kLaneThreads];
     const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
     if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    const size_t base = (size_t)n * t.k * in.S + s;
-    if (t.valid && !t.valid[r]) return put(loss, stats, in.rows, r, 0.f, kNoStats);
-    const Target g = target_of(t, in.C, base, in.S, r);
-    if (!g.any) return put(loss, stats, in.rows, r, 0.f, kNoStats);
-    LogSum out = {-INFINITY, 0.f}, top = {-INFINITY, 0.f};
-    for (int c0 = 0; c0 < in.C; c0 += 32 * kChunkWords) {
-        const int c1 = min(in.C, c0 + 32 * kChunkWords);
-        if (REST) {
-            for (int w = 0; w < kChunkWords; ++w) marks[w][threadIdx.x] = 0;
-            for (int j = 0; j < t.k; ++j) {
-                const int i = t.labels[base + (size_t)j * in.S];
-                if (i < c0 || i >= c1) continue;
-                const uint32_t bit = 1u << ((i - c0) & 31), old = marks[(i - c0) >> 5][threadIdx.x];
-                if (!(old & bit)) {     // a label named twice counts once on the student's side
-                    marks[(i - c0) >> 5][threadIdx.x] = old | bit;
-                    add_score(top, to_float(p[i * in.sc]), t.c2);
-                }
-            }
-        }
-        for (int c = c0; c < c1; c += 32) {
-            const uint32_t word = REST ? marks[(c - c0) >> 5][threadIdx.x] : 0;
-            const int end = min(32, c1 - c);
-            constexpr int U = 8;
-            const T *q = p + c * in.sc;
-            int i = 0;
-            for (; i + U <= end; i += U) {
-                float x[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = to_float(q[(i + u) * in.sc]);
-                float m = out.m;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (REST && (word >> (i + u) & 1)) x[u] = -INFINITY;
-                    m = fmaxf(m, x[u]);
-                }
-                const float ref = finite_or_zero(m);
-                float sum = out.s * __builtin_amdgcn_exp2f((out.m - ref) * t.c2);
-#pragma unroll
-                for (int u = 0; u < U; ++u) sum += __builtin_amdgcn_exp2f((x[u] - ref) * t.c2);
-                out = {m, sum};
-            }
-            for (; i < end; ++i)
-                if (!(REST && (word >> i & 1))) add_score(out, to_float(q[i * in.sc]), t.c2);
-        }
+    // (everything is asked for before anything is looked at)
+    LaneRecord<T, KB, ALL> record(in, t, p, (size_t)n * t.k * in.S + s);
+    float x[CB];
+    load_labels(x, in, p, 0);
+    const RowFlags flags(t, r);
+    record.fetch();
+    LogSum out = {-INFINITY, 0.f};
+    Excess top = kNoExcess;
+    for (int c0 = 0;;) {
+        add_labels(record, x, c0, t.c2, out, top);
+        c0 += CB;
+        if (LONE || c0 >= in.C) break;
+        load_labels(x, in, p, c0);
     }
-    const LogSum all = REST ? join(out, top, t.c2) : out;
-    const Stats a = stats_of(all, out, REST);
-    if (a.m == -INFINITY) return put(loss, stats, in.rows, r, 0.f, a);
-    float sum = REST ? share_term(g.p_rest, g.log_p_rest, log_q_rest(a, t.inv_t)) : 0.f;
-    for (int j = 0; j < t.k; ++j) {
-        const int i = t.labels[base + (size_t)j * in.S];
-        if ((unsigned)i >= (unsigned)in.C) continue;
-        const float lp = (load_any(t.values, t.dtype, base + (size_t)j * in.S) - g.sum.m) * t.inv_t - g.log_a;
-        const float lq = (to_float(p[i * in.sc]) - a.m) * t.inv_t - a.z;
-        sum += share_term(__builtin_amdgcn_exp2f(lp * kLog2e), lp, lq);
-    }
-    put(loss, stats, in.rows, r, t.t * t.t * sum, a);
+    const Target g = record.target(flags.rest(t));
+    const Stats a = stats_of(top, out, t.c2);
+    if (!flags.valid(t) || !g.any || a.m == -INFINITY) return put(loss, LONE ? nullptr : stats, in.rows, r, 0.f, kNoStats);
+    float sum = t.rest ? share_term(g.p_rest, g.log_p_rest, log_q_rest(a, t.inv_t)) : 0.f;
+    record.each([&](const Block<T, KB> &b) {
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+            const float lp = log_share(t, g, b.value[j]), lq = (b.x[j] - a.m) * t.inv_t - a.z;
+            sum += b.label[j] >= 0 ? share_term(__builtin_amdgcn_exp2f(lp * kLog2e), lp, lq) : 0.f;
+        }
+    });
+    put(loss, LONE ? nullptr : stats, in.rows, r, t.t * t.t * sum, a);
 }
 
-// Gradient of the scores.  What the record takes from a label lies in LDS, one column of 32 labels per lane (-1: not named).
-template <typename T>
+// What the record takes from each label of a block lies in LDS, one column per lane (-1: not named).
+template <typename T, int CB, bool LONE, int KB, bool ALL>
 __global__ void __launch_bounds__(kLaneThreads)
 backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const float *__restrict__ grad_loss, T *__restrict__ grad,
                       long long gn, long long gc, long long gs)
 {
-    __shared__ float taken[32][kLaneThreads];
+    __shared__ float taken[CB][kLaneThreads];
     const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
     if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
     T *out = grad + (long long)n * gn + (long long)s * gs;
-    const size_t base = (size_t)n * t.k * in.S + s;
-    const Stats a = load_stats(stats, in.rows, r);
-    Target g;
-    g.any = false;
-    if (!(t.valid && !t.valid[r]) && a.m != -INFINITY) g = target_of(t, in.C, base, in.S, r);
-    if (!g.any) {
+    LaneRecord<T, KB, ALL> record(in, t, p, (size_t)n * t.k * in.S + s);
+    float x[CB];
+    load_labels(x, in, p, 0);
+    const RowFlags flags(t, r);
+    const float up = grad_loss[r];
+    record.fetch();
+    Stats a;
+    if constexpr (LONE) {
+        LogSum other = {-INFINITY, 0.f};
+        Excess top = kNoExcess;
+        add_labels(record, x, 0, t.c2, other, top);
+        a = stats_of(top, other, t.c2);
+    } else {
+        a = load_stats(stats, in.rows, r);
+    }
+    const Target g = record.target(flags.rest(t));
+    if (!flags.valid(t) || a.m == -INFINITY || !g.any) {
         for (int c = 0; c < in.C; ++c) from_float(0.f, out[c * gc]);
         return;
     }
-    const Slope sl = slope_of(a, t, g, grad_loss[r]);
-    for (int i = 0; i < 32; ++i) taken[i][threadIdx.x] = -1.f;
-    for (int c0 = 0; c0 < in.C; c0 += 32) {
-        const int end = min(32, in.C - c0);
-        for (int j = 0; j < t.k; ++j) {
-            const int i = t.labels[base + (size_t)j * in.S] - c0;
-            if (i < 0 || i >= end) continue;
-            const float lp = (load_any(t.values, t.dtype, base + (size_t)j * in.S) - g.sum.m) * t.inv_t - g.log_a;
-            taken[i][threadIdx.x] = fmaxf(taken[i][threadIdx.x], 0.f) + __builtin_amdgcn_exp2f(lp * kLog2e);
-        }
-        const T *q = p + c0 * in.sc;
+    const Slope sl = slope_of(a, t, g, up);
+#pragma unroll
+    for (int i = 0; i < CB; ++i) taken[i][threadIdx.x] = -1.f;
+    for (int c0 = 0; c0 < (LONE ? 1 : in.C); c0 += CB) {
+        if (c0) load_labels(x, in, p, c0);
+        record.each([&](const Block<T, KB> &b) {
+#pragma unroll
+            for (int j = 0; j < KB; ++j) {
+                const int i = b.label[j] - c0;
+                if (b.label[j] < 0 || (unsigned)i >= (unsigned)CB) continue;
+                taken[i][threadIdx.x] = fmaxf(taken[i][threadIdx.x], 0.f) + __builtin_amdgcn_exp2f(log_share(t, g, b.value[j]) * kLog2e);
+            }
+        });
         T *w = out + c0 * gc;
-        for (int i = 0; i < end; ++i) {
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
             const float share = taken[i][threadIdx.x];
-            from_float(slope(sl, to_float(q[i * in.sc]), share, t.c2), w[i * gc]);
+            if (c0 + i < in.C) from_float(slope(sl, x[i], share, t.c2), w[i * gc]);
             if (share >= 0.f) taken[i][threadIdx.x] = -1.f;
         }
     }
 }
 
+// ---- one or more workgroups per row (class stride 1)
+//
+// Rows of many labels are cut into parts, as many as it takes to have work for the whole card: a part's running sum over
+// the labels outside the record goes to the workspace, and one wave per row joins them and adds the record's side.
+
 constexpr int kRowThreads = 256;
 constexpr int kSegment = 1 << 16;       // labels marked at a time by a workgroup: 8 KB of bits
+constexpr int kMaxParts = 64;
+constexpr int kMinPart = 8192;
 
-__device__ inline LogSum block_join(LogSum a, LogSum (*part)[2], int which, float c)
+__host__ __device__ inline int part_labels(int C, int parts) { return (((C + parts - 1) / parts) + 2047) & ~2047; }
+int parts_of(const Rows &in, unsigned enough)
 {
-    a = wave_join(a, c);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][which] = a;
-    __syncthreads();
-    a = part[0][which];
-    for (int w = 1; w < kRowThreads / 64; ++w) a = join(a, part[w][which], c);
-    return a;
+    const unsigned most = (unsigned)((in.C + kMinPart - 1) / kMinPart), want = (enough + in.rows - 1) / in.rows;
+    const unsigned n = want < most ? want : most;
+    return (int)(n < 1 ? 1 : n > kMaxParts ? kMaxParts : n);
 }
 
-template <typename T, bool REST>
-__global__ void __launch_bounds__(kRowThreads)
-forward_rows_kernel(Rows in, Teacher t, float *__restrict__ loss, float *__restrict__ stats)
+// Marks the record's labels in [c0, c1) as bits
+__device__ inline void mark(uint32_t *bits, const Teacher &t, size_t base, size_t step, int c0, int c1)
 {
-    extern __shared__ uint32_t bits[];
-    __shared__ LogSum part[kRowThreads / 64][2];
-    const unsigned r = blockIdx.x;
-    const unsigned n = r / in.S, s = r - n * in.S;
-    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    const size_t base = (size_t)n * t.k * in.S + s;
-    float l = 0.f;
-    Stats a = kNoStats;
-    bool live = !(t.valid && !t.valid[r]);
-    Target g;
-    if (live) {
-        g = target_of(t, in.C, base, in.S, r);      // (every lane the same; k entries)
-        live = g.any;
+    for (int w = threadIdx.x; w < (c1 - c0 + 31) / 32; w += kRowThreads) bits[w] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < t.k; j += kRowThreads) {
+        const int i = t.labels[base + (size_t)j * step];
+        if (i >= c0 && i < c1) atomicOr(&bits[(i - c0) >> 5], 1u << ((i - c0) & 31));
     }
-    if (live) {
-        LogSum out = {-INFINITY, 0.f}, top = {-INFINITY, 0.f};
-        for (int c0 = 0; c0 < in.C; c0 += kSegment) {
-            const int c1 = min(in.C, c0 + kSegment);
-            if (REST) {
-                __syncthreads();
-                for (int w = threadIdx.x; w < (c1 - c0 + 31) / 32; w += kRowThreads) bits[w] = 0;
-                __syncthreads();
-                for (int j = threadIdx.x; j < t.k; j += kRowThreads) {
-                    const int i = t.labels[base + (size_t)j * in.S];
-                    if (i < c0 || i >= c1) continue;
-                    const uint32_t bit = 1u << ((i - c0) & 31);
-                    // (a label named twice counts once on the student's side)
-                    if (!(atomicOr(&bits[(i - c0) >> 5], bit) & bit)) add_score(top, to_float(p[i * in.sc]), t.c2);
-                }
-                __syncthreads();
-            }
-            for (int c = c0 + threadIdx.x; c < c1; c += kRowThreads)
-                if (!(REST && (bits[(c - c0) >> 5] >> ((c - c0) & 31) & 1))) add_score(out, to_float(p[c * in.sc]), t.c2);
-        }
-        out = block_join(out, part, 0, t.c2);
-        LogSum all = out;
-        if (REST) {
-            top = block_join(top, part, 1, t.c2);
-            all = join(out, top, t.c2);
-        }
-        a = stats_of(all, out, REST);
-        if (a.m != -INFINITY && threadIdx.x == 0) {
-            float sum = REST ? share_term(g.p_rest, g.log_p_rest, log_q_rest(a, t.inv_t)) : 0.f;
-            for (int j = 0; j < t.k; ++j) {
-                const int i = t.labels[base + (size_t)j * in.S];
-                if ((unsigned)i >= (unsigned)in.C) continue;
-                const float lp = (load_any(t.values, t.dtype, base + (size_t)j * in.S) - g.sum.m) * t.inv_t - g.log_a;
-                const float lq = (to_float(p[i * in.sc]) - a.m) * t.inv_t - a.z;
-                sum += share_term(__builtin_amdgcn_exp2f(lp * kLog2e), lp, lq);
-            }
-            l = t.t * t.t * sum;
-        }
-    }
-    if (threadIdx.x == 0) put(loss, stats, in.rows, r, l, a);
+    __syncthreads();
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-backward_rows_kernel(Rows in, Teacher t, const float *__restrict__ stats, const float *__restrict__ grad_loss, T *__restrict__ grad,
-                     long long gn, long long gc, long long gs)
+outside_parts_kernel(Rows in, Teacher t, int parts, LogSum *__restrict__ sums)
 {
+    extern __shared__ uint32_t bits[];
+    __shared__ LogSum wave_sum[kRowThreads / 64];
+    constexpr int V = kVec<T>;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const unsigned n = r / in.S, s = r - n * in.S;
+    if (t.valid && !t.valid[r]) return;
+    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
+    const size_t base = (size_t)n * t.k * in.S + s;
+    const int size = part_labels(in.C, parts);
+    const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
+    LogSum out = {-INFINITY, 0.f};
+    for (int c0 = begin; c0 < end; c0 += kSegment) {
+        const int c1 = min(end, c0 + kSegment);
+        if (c0 > begin) __syncthreads();
+        mark(bits, t, base, in.S, c0, c1);
+        auto take = [&](float (&x)[V], int c) {
+            const uint32_t marks = ((const uint8_t *)bits)[(c - c0) >> 3] >> (V == 4 ? (c - c0) & 4 : 0);
+            if (marks) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = marks >> i & 1 ? -INFINITY : x[i];
+            }
+            float m = out.m;
+#pragma unroll
+            for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+            const float ref = finite_or_zero(m);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * t.c2);
+            out = {m, fmaf(out.s, __builtin_amdgcn_exp2f((out.m - ref) * t.c2), sum)};
+        };
+        constexpr int U = 4;            // vectors in flight
+        int c = c0 + threadIdx.x * V;
+        for (; c + (U - 1) * kRowThreads * V + V <= c1; c += U * kRowThreads * V) {
+            float x[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_vec(p + c + u * kRowThreads * V, x[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) take(x[u], c + u * kRowThreads * V);
+        }
+        for (; c < c1; c += kRowThreads * V) {
+            float x[V];
+            if (c + V <= c1) {
+                load_vec(p + c, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = c + i < c1 ? to_float(p[c + i]) : -INFINITY;
+            }
+            take(x, c);
+        }
+    }
+    out = wave_join(out, t.c2);
+    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = out;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kRowThreads / 64; ++w) out = join(out, wave_sum[w], t.c2);
+        sums[blockIdx.x] = out;
+    }
+}
+
+// A row's record over the lanes of a wave, entries lane and lane + 64
+struct Entries {
+    int label[2];
+    float value[2];
+    bool in[2];                 // a label of the row
+};
+__device__ inline Entries entries_of(const Teacher &t, int C, size_t base, size_t step, int lane)
+{
+    Entries e;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int j = lane + 64 * h;
+        e.label[h] = j < t.k ? t.labels[base + (size_t)j * step] : -1;
+        e.in[h] = (unsigned)e.label[h] < (unsigned)C;
+    }
+    load_any(e.value, t.values, t.dtype, [&](int h) { return base + (size_t)min(lane + 64 * h, t.k - 1) * step; });
+    return e;
+}
+__device__ inline Target target_by_wave(const Teacher &t, const Entries &e, unsigned r)
+{
+    Excess sum = kNoExcess;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (e.in[h]) sum = join(sum, Excess{e.value[h], 0.f}, t.c2);
+    const bool named = __any(e.in[0] || e.in[1]);
+    return target_of(t, wave_join(sum, t.c2), named, t.rest ? t.rest[r] : -INFINITY);
+}
+
+// One wave per row
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+finish_rows_kernel(Rows in, Teacher t, int parts, const LogSum *__restrict__ sums, float *__restrict__ loss, float *__restrict__ stats)
+{
+    __shared__ int labels[kRowThreads / 64][MFL_MAX_TOP_LABELS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned r = blockIdx.x * (kRowThreads / 64) + wave;
+    if (r >= in.rows) return;
+    const unsigned n = r / in.S, s = r - n * in.S;
+    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
+    const size_t base = (size_t)n * t.k * in.S + s;
+    if (t.valid && !t.valid[r]) {
+        if (lane == 0) put(loss, stats, in.rows, r, 0.f, kNoStats);
+        return;
+    }
+    const Entries e = entries_of(t, in.C, base, in.S, lane);
+    float x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        x[h] = e.in[h] ? to_float(p[e.label[h]]) : -INFINITY;
+        labels[wave][lane + 64 * h] = e.label[h];
+    }
+    LogSum out = lane < parts ? sums[(size_t)r * parts + lane] : LogSum{-INFINITY, 0.f};
+    out = wave_join(out, t.c2);
+    const Target g = target_by_wave(t, e, r);
+    if (!g.any) {
+        if (lane == 0) put(loss, stats, in.rows, r, 0.f, kNoStats);
+        return;
+    }
+    // the record's labels on the student's side: each once, by the first entry that names it
+    __builtin_amdgcn_wave_barrier();
+    bool again[2] = {false, false};
+    for (int j = 0; j < t.k; ++j) {
+        const int l = labels[wave][j];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) again[h] |= j < lane + 64 * h && l == e.label[h];
+    }
+    Excess top = kNoExcess;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (e.in[h] && !again[h]) top = join(top, Excess{x[h], 0.f}, t.c2);
+    top = wave_join(top, t.c2);
+    const Stats a = stats_of(top, out, t.c2);
+    if (a.m == -INFINITY) {
+        if (lane == 0) put(loss, stats, in.rows, r, 0.f, a);
+        return;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (!e.in[h]) continue;
+        const float lp = log_share(t, g, e.value[h]), lq = (x[h] - a.m) * t.inv_t - a.z;
+        sum += share_term(__builtin_amdgcn_exp2f(lp * kLog2e), lp, lq);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (t.rest) sum += share_term(g.p_rest, g.log_p_rest, log_q_rest(a, t.inv_t));
+    if (lane == 0) put(loss, stats, in.rows, r, t.t * t.t * sum, a);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+backward_rows_kernel(Rows in, Teacher t, int parts, const float *__restrict__ stats, const float *__restrict__ grad_loss,
+                     T *__restrict__ grad, long long gn, long long gs)
+{
+    extern __shared__ uint32_t bits[];
     __shared__ int label[MFL_MAX_TOP_LABELS];
     __shared__ float share[MFL_MAX_TOP_LABELS];
-    const unsigned r = blockIdx.x;
+    constexpr int V = kVec<T>;
+    const int lane = threadIdx.x & 63;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
     T *out = grad + (long long)n * gn + (long long)s * gs;
     const size_t base = (size_t)n * t.k * in.S + s;
+    const int size = part_labels(in.C, parts);
+    const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
     const Stats a = load_stats(stats, in.rows, r);
     Target g;
     g.any = false;
-    if (!(t.valid && !t.valid[r]) && a.m != -INFINITY) g = target_of(t, in.C, base, in.S, r);
+    if (!(t.valid && !t.valid[r]) && a.m != -INFINITY) {
+        const Entries e = entries_of(t, in.C, base, in.S, lane);
+        g = target_by_wave(t, e, r);
+        if (threadIdx.x < 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                label[lane + 64 * h] = e.label[h];
+                share[lane + 64 * h] = e.in[h] ? __builtin_amdgcn_exp2f(log_share(t, g, e.value[h]) * kLog2e) : 0.f;
+            }
+        }
+    }
     if (!g.any) {
-        for (int c = threadIdx.x; c < in.C; c += kRowThreads) from_float(0.f, out[c * gc]);
+        const float zero[V] = {};
+        for (int c = begin + threadIdx.x * V; c < end; c += kRowThreads * V) {
+            if (c + V <= end) {
+                store_vec(out + c, zero);
+            } else {
+                for (int i = c; i < end; ++i) from_float(0.f, out[i]);
+            }
+        }
         return;
     }
-    for (int j = threadIdx.x; j < t.k; j += kRowThreads) {
-        label[j] = t.labels[base + (size_t)j * in.S];
-        share[j] = __builtin_amdgcn_exp2f(((load_any(t.values, t.dtype, base + (size_t)j * in.S) - g.sum.m) * t.inv_t - g.log_a) * kLog2e);
-    }
-    __syncthreads();
     const Slope sl = slope_of(a, t, g, grad_loss[r]);
-    for (int c = threadIdx.x; c < in.C; c += kRowThreads) {
-        float taken = -1.f;
-        for (int j = 0; j < t.k; ++j)
-            if (label[j] == c) taken = fmaxf(taken, 0.f) + share[j];
-        from_float(slope(sl, to_float(p[c * in.sc]), taken, t.c2), out[c * gc]);
+    for (int c0 = begin; c0 < end; c0 += kSegment) {
+        const int c1 = min(end, c0 + kSegment);
+        __syncthreads();
+        mark(bits, t, base, in.S, c0, c1);
+        auto turn = [&](float (&x)[V], int c) {
+            const uint32_t marks = ((const uint8_t *)bits)[(c - c0) >> 3] >> (V == 4 ? (c - c0) & 4 : 0);
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[i] = sl.f_out * __builtin_amdgcn_exp2f(fmaf(x[i] - sl.m_out, t.c2, sl.o_out));
+            if (marks & ((1 << V) - 1)) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (!(marks >> i & 1)) continue;
+                    float sum = 0.f;
+                    for (int j = 0; j < t.k; ++j) sum += label[j] == c + i ? share[j] : 0.f;
+                    y[i] = slope(sl, x[i], sum, t.c2);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = y[i];
+        };
+        constexpr int U = 4;
+        int c = c0 + threadIdx.x * V;
+        for (; c + (U - 1) * kRowThreads * V + V <= c1; c += U * kRowThreads * V) {
+            float x[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_vec(p + c + u * kRowThreads * V, x[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                turn(x[u], c + u * kRowThreads * V);
+                store_vec(out + c + u * kRowThreads * V, x[u]);
+            }
+        }
+        for (; c < c1; c += kRowThreads * V) {
+            float x[V];
+            if (c + V <= c1) {
+                load_vec(p + c, x);
+                turn(x, c);
+                store_vec(out + c, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = c + i < c1 ? to_float(p[c + i]) : 0.f;
+                turn(x, c);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (c + i < c1) from_float(x[i], out[c + i]);
+            }
+        }
     }
 }
 
 bool by_rows(const Rows &in) { return in.sc == 1 && in.C >= 512; }
+size_t mark_bytes(int C, int parts)
+{
+    const int size = part_labels(C, parts);
+    return (size_t)(size < kSegment ? size : kSegment) / 8;
+}
+constexpr unsigned kEnough = 2048;      // workgroups that fill the card: 256 CUs, eight each
+
+// labels and entries a lane takes at a time
+#define MFL_BY_SIZE(C, k, LAUNCH)                                                             \
+    do {                                                                                      \
+        if (C <= 8) {                                                                         \
+            if (k <= 4) LAUNCH(8, true, 4, true);                                             \
+            else LAUNCH(8, true, 8, false);                                                   \
+        } else if (C <= kLoneBlock) {                                                         \
+            if (k <= 4) LAUNCH(kLoneBlock, true, 4, true);                                    \
+            else LAUNCH(kLoneBlock, true, 8, false);                                          \
+        } else {                                                                              \
+            if (k <= 4) LAUNCH(32, false, 4, true);                                           \
+            else if (k <= 8) LAUNCH(32, false, 8, true);                                      \
+            else LAUNCH(32, false, 8, false);                                                 \
+        }                                                                                     \
+    } while (0)
 
 template <typename T>
-int run_forward(const Rows &in, const Teacher &t, float *loss, float *stats, hipStream_t st)
+int run_forward(const Rows &in, const Teacher &t, float *loss, float *stats, void *workspace, hipStream_t st)
 {
     if (by_rows(in)) {
-        const size_t lds = t.rest ? (size_t)((in.C < kSegment ? in.C : kSegment) + 31) / 32 * 4 : 0;
-        if (t.rest) hipLaunchKernelGGL((forward_rows_kernel<T, true>), dim3(in.rows), dim3(kRowThreads), lds, st, in, t, loss, stats);
-        else hipLaunchKernelGGL((forward_rows_kernel<T, false>), dim3(in.rows), dim3(kRowThreads), lds, st, in, t, loss, stats);
-    } else {
-        const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
-        if (t.rest) hipLaunchKernelGGL((forward_lanes_kernel<T, true>), grid, block, 0, st, in, t, loss, stats);
-        else hipLaunchKernelGGL((forward_lanes_kernel<T, false>), grid, block, 0, st, in, t, loss, stats);
+        const int parts = parts_of(in, kEnough);
+        hipLaunchKernelGGL(outside_parts_kernel<T>, dim3(in.rows * parts), dim3(kRowThreads), mark_bytes(in.C, parts), st, in, t, parts,
+                           (LogSum *)workspace);
+        const unsigned per = kRowThreads / 64;
+        hipLaunchKernelGGL(finish_rows_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kRowThreads), 0, st, in, t, parts,
+                           (const LogSum *)workspace, loss, stats);
+        return (int)hipGetLastError();
     }
+    const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
+#define MFL_LANES(CB, LONE, KB, ALL) \
+    hipLaunchKernelGGL((forward_lanes_kernel<T, CB, LONE, KB, ALL>), grid, block, 0, st, in, t, loss, stats)
+    MFL_BY_SIZE(in.C, t.k, MFL_LANES);
+#undef MFL_LANES
     return (int)hipGetLastError();
 }
 
 template <typename T>
-int run_backward(const Rows &in, const Teacher &t, const float *stats, const float *grad_loss, void *grad, long long gn, long long gc,
-                 long long gs, hipStream_t st)
+int run_backward(const Rows &in, const Teacher &t, const float *stats, const float *grad_loss, void *grad, const Rows &out, hipStream_t st)
 {
-    if (by_rows(in)) {
-        hipLaunchKernelGGL(backward_rows_kernel<T>, dim3(in.rows), dim3(kRowThreads), 0, st, in, t, stats, grad_loss, (T *)grad, gn, gc, gs);
-    } else {
-        const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
-        hipLaunchKernelGGL(backward_lanes_kernel<T>, grid, block, 0, st, in, t, stats, grad_loss, (T *)grad, gn, gc, gs);
+    if (by_rows(in) && out.sc == 1) {
+        const int parts = parts_of(in, kEnough);
+        hipLaunchKernelGGL(backward_rows_kernel<T>, dim3(in.rows * parts), dim3(kRowThreads), mark_bytes(in.C, parts), st, in, t, parts,
+                           stats, grad_loss, (T *)grad, out.sn, out.ss);
+        return (int)hipGetLastError();
     }
+    const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
+#define MFL_LANES(CB, LONE, KB, ALL) \
+    hipLaunchKernelGGL((backward_lanes_kernel<T, CB, LONE, KB, ALL>), grid, block, 0, st, in, t, stats, grad_loss, (T *)grad, out.sn, out.sc, \
+                       out.ss)
+    MFL_BY_SIZE(in.C, t.k, MFL_LANES);
+#undef MFL_LANES
     return (int)hipGetLastError();
 }
 
@@ -386,10 +682,12 @@ int make_teacher(Teacher &t, const void *values, int dtype, const int *labels, c
 
 extern "C" {
 
+// (for any strides: a size that the lanes serve is not worth telling apart)
 size_t mfl_distillation_workspace_bytes(int N, int C, int S, int dtype, int k)
 {
-    (void)N, (void)C, (void)S, (void)dtype, (void)k;
-    return 0;
+    Rows in;
+    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || k < 1 || C < 512) return 0;
+    return (size_t)in.rows * parts_of(in, kEnough) * sizeof(LogSum);
 }
 
 int mfl_distillation_forward(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c,
@@ -403,13 +701,12 @@ int mfl_distillation_forward(const void *scores, int dtype, int N, int C, int S,
     if (!rc) rc = make_teacher(t, values, values_dtype, labels, rest, valid, k, temperature);
     if (rc) return rc;
     if (!loss || !stats) return MFL_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < mfl_distillation_workspace_bytes(N, C, S, dtype, k)) return MFL_ERR_WORKSPACE;
-    (void)workspace;
+    if (by_rows(in) && (!workspace || workspace_bytes < mfl_distillation_workspace_bytes(N, C, S, dtype, k))) return MFL_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case MFL_F32: return run_forward<float>(in, t, loss, stats, st);
-    case MFL_BF16: return run_forward<bf16_t>(in, t, loss, stats, st);
-    default: return run_forward<f16_t>(in, t, loss, stats, st);
+    case MFL_F32: return run_forward<float>(in, t, loss, stats, workspace, st);
+    case MFL_BF16: return run_forward<bf16_t>(in, t, loss, stats, workspace, st);
+    default: return run_forward<f16_t>(in, t, loss, stats, workspace, st);
     }
 }
 
@@ -427,9 +724,9 @@ int mfl_distillation_backward(const void *scores, int dtype, int N, int C, int S
     if (!stats || !grad_loss) return MFL_ERR_INVALID_ARGUMENT;
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case MFL_F32: return run_backward<float>(in, t, stats, grad_loss, d_scores, out.sn, out.sc, out.ss, st);
-    case MFL_BF16: return run_backward<bf16_t>(in, t, stats, grad_loss, d_scores, out.sn, out.sc, out.ss, st);
-    default: return run_backward<f16_t>(in, t, stats, grad_loss, d_scores, out.sn, out.sc, out.ss, st);
+    case MFL_F32: return run_backward<float>(in, t, stats, grad_loss, d_scores, out, st);
+    case MFL_BF16: return run_backward<bf16_t>(in, t, stats, grad_loss, d_scores, out, st);
+    default: return run_backward<f16_t>(in, t, stats, grad_loss, d_scores, out, st);
     }
 }
 

@@ -32,18 +32,58 @@ __device__ inline float to_float(f16_t v) { return (float)v.h; }
 // one rounding, to nearest even; a NaN stays one
 __device__ inline void from_float(float v, float &o) { o = v; }
 __device__ inline void from_float(float v, f16_t &o) { o.h = (_Float16)v; }
-__device__ inline void from_float(float v, bf16_t &o)
+__device__ inline void from_float(float v, bf16_t &o) { o.u = __builtin_bit_cast(uint16_t, (__bf16)v); }
+
+// 16 bytes of scores at any address of their type (the hardware takes unaligned vector accesses)
+typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+typedef words4 words4_at2 __attribute__((aligned(2)));
+template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
+template <typename T> __device__ inline void load_vec(const T *p, float (&x)[kVec<T>])
 {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    o.u = (u & 0x7fffffffu) > 0x7f800000u ? (uint16_t)((u >> 16) | 0x40u) : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+    const words4 w = *(const words4_at2 *)p;
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) {
+        // (a copy: a bit cast of a vector's element takes its first one)
+        const uint32_t u = w[sizeof(T) == 4 ? i : i / 2];
+        if constexpr (sizeof(T) == 4) x[i] = __builtin_bit_cast(float, u);
+        else x[i] = to_float(__builtin_bit_cast(T, (uint16_t)(u >> (16 * (i & 1)))));
+    }
+}
+template <typename T> __device__ inline void store_vec(T *p, const float (&x)[kVec<T>])
+{
+    words4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __builtin_bit_cast(uint32_t, x[i]);
+        } else {
+            T lo, hi;
+            from_float(x[2 * i], lo);
+            from_float(x[2 * i + 1], hi);
+            w[i] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | (uint32_t)__builtin_bit_cast(uint16_t, hi) << 16;
+        }
+    }
+    *(words4_at2 *)p = w;
 }
 
-// a value of a tensor whose type is known at run time only (uniform branch; the teacher's k values of a row)
-__device__ inline float load_any(const void *p, int dtype, size_t i)
+// Values of a tensor whose type is known at run time only (the teacher's side): all bits first, so that the loads of a
+// block are in flight together, then the conversion
+template <int N, typename At> __device__ inline void load_any(float (&v)[N], const void *p, int dtype, At at)
 {
-    if (dtype == MFL_F32) return ((const float *)p)[i];
-    if (dtype == MFL_BF16) return to_float(((const bf16_t *)p)[i]);
-    return to_float(((const f16_t *)p)[i]);
+    uint32_t raw[N];
+    if (dtype == MFL_F32) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) raw[j] = ((const uint32_t *)p)[at(j)];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) raw[j] = ((const uint16_t *)p)[at(j)];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float h = (float)__builtin_bit_cast(_Float16, (uint16_t)raw[j]);
+        const float b = __builtin_bit_cast(float, dtype == MFL_BF16 ? raw[j] << 16 : raw[j]);
+        v[j] = dtype == MFL_F16 ? h : b;
+    }
 }
 
 // Order of scores as signed integers: -inf < ... < -0 = +0 < ... < +inf < NaN
@@ -86,6 +126,34 @@ __device__ inline LogSum wave_join(LogSum a, float c)
         a = join(a, b, c);
     }
     return a;
+}
+
+// (m, s) stands for (1 + s) * exp(m), m the largest term: where one term outweighs all others, 1 + s would keep nothing of
+// them in fp32, and -log of that term's share, log1p(s), is just what a confident row's loss consists of.  m = -inf, s = -1:
+// nothing yet.
+struct Excess {
+    float m, s;
+};
+constexpr Excess kNoExcess = {-INFINITY, -1.f};
+__device__ inline Excess join(Excess a, Excess b, float c)
+{
+    const bool first = a.m >= b.m;
+    const float ref = finite_or_zero(first ? a.m : b.m);
+    const Excess hi = first ? a : b, lo = first ? b : a;
+    return {hi.m, fmaf(1.f + lo.s, __builtin_amdgcn_exp2f((lo.m - ref) * c), hi.s)};
+}
+__device__ inline Excess wave_join(Excess a, float c)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = join(a, Excess{__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, c);
+    return a;
+}
+
+// log(1 + s) for s >= -1 to a few steps: log(u) of the rounded u = 1 + s, scaled by the part of s that u keeps (Kahan)
+__device__ inline float log_1p(float s)
+{
+    const float u = 1.f + s, kept = u - 1.f;
+    return kept == 0.f || u == INFINITY ? s : logf(u) * (s * __builtin_amdgcn_rcpf(kept));
 }
 
 // log(s * exp(m / temperature)); -inf for nothing, and an infinite score stays infinite

@@ -168,66 +168,102 @@ def argmax_labels(logq: torch.Tensor) -> torch.Tensor:
 
 
 def _score_rows(t: torch.Tensor, name: str = "scores"):
-    """[N, C] or [N, C, ...] scores as the library reads them: (tensor to keep alive, dtype code, N, C, S, three strides).
-    Nothing is copied where the dimensions behind C have one common stride (contiguous and channels-last maps, slices)."""
-    if t.dim() < 2:
-        raise RuntimeError(f"{name} must be [N, C] or [N, C, ...], got {tuple(t.shape)}")
-    if t.numel() == 0:
-        raise RuntimeError(f"{name} is empty: {tuple(t.shape)}")
+    """[N, C] or [N, C, ...] scores as the library reads them: (tensor to keep alive, (address, dtype code, N, C, S, three
+    strides)).  Nothing is copied where the dimensions behind C have one common stride (contiguous and channels-last maps,
+    slices)."""
+    if not t.is_cuda:
+        raise RuntimeError(f"semantic_segmentation_amd runs on a ROCm GPU only: got a tensor on '{t.device}' (there is no CPU "
+                           "fallback)")
+    code = _lib.SCORE_DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    shape = t.shape
+    if len(shape) < 2:
+        raise RuntimeError(f"{name} must be [N, C] or [N, C, ...], got {tuple(shape)}")
+    total = t.numel()
+    if total == 0:
+        raise RuntimeError(f"{name} is empty: {tuple(shape)}")
+    N, C = shape[0], shape[1]
+    if t.is_contiguous():
+        S = total // (N * C)
+        return t, (t.data_ptr(), code, N, C, S, C * S, S, 1)
     v = t.detach()
-    v = v.unsqueeze(2) if v.dim() == 2 else v.flatten(2)
-    return v, (_lib.SCORE_DTYPES[t.dtype],) + tuple(v.shape) + tuple(v.stride())
+    v = v.unsqueeze(2) if len(shape) == 2 else v.flatten(2)
+    return v, (v.data_ptr(), code) + tuple(v.shape) + tuple(v.stride())
 
 
-def _like_rows(t: torch.Tensor, x, name: str, dtypes, shape):
-    """A tensor beside the scores: its device, type and shape checked, contiguous."""
-    if not x.is_cuda or x.device != t.device:
+def _beside(t: torch.Tensor, x, name: str, dtypes, shape):
+    """A tensor that goes with the scores: its device, type and shape checked, contiguous."""
+    if x.get_device() != t.get_device():
         raise RuntimeError(f"{name} must be on {t.device}, got {x.device}")
     if x.dtype not in dtypes:
         raise RuntimeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {x.dtype}")
-    if tuple(x.shape) != tuple(shape):
+    if x.shape != shape:
         raise RuntimeError(f"{name} must be {tuple(shape)}, got {tuple(x.shape)}")
-    return x.detach().contiguous()
+    return x if x.is_contiguous() else x.detach().contiguous()
 
 
-def _score_workspace(n: int, t: torch.Tensor):
-    return torch.empty(n, dtype=torch.uint8, device=t.device) if n else None
+def _address(x):
+    return None if x is None else x.data_ptr()
+
+
+_F32, _I32, _FLAGS = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
 
 
 def top_labels(scores: torch.Tensor, k: int, temperature: float = 1.0):
     """The k largest scores of every row of [N, C] or [N, C, ...] scores, descending, the lower label first among equals:
     (values [N, k, ...] of the scores' type, labels [N, k, ...] int32, rest [N, ...] float32), with rest = log sum
     exp(score / temperature) over all other labels (-inf if there are none).  The record distillation_forward reads."""
-    _lib.require_scores(scores)
     v, args = _score_rows(scores)
-    if not 1 <= k <= min(args[2], _lib.MAX_TOP_LABELS):
-        raise ValueError(f"k must be between 1 and min(C, {_lib.MAX_TOP_LABELS}), got {k} with C = {args[2]}")
-    shape = tuple(scores.shape)
-    values = torch.empty((shape[0], k) + shape[2:], dtype=scores.dtype, device=scores.device)
-    labels = torch.empty((shape[0], k) + shape[2:], dtype=torch.int32, device=scores.device)
-    rest = torch.empty((shape[0],) + shape[2:], dtype=torch.float32, device=scores.device)
-    with torch.cuda.device(scores.device):
-        n = int(lib.mfl_top_labels_workspace_bytes(args[1], args[2], args[3], args[0], k))
-        ws = _score_workspace(n, scores)
-        _lib.check(lib.mfl_top_labels(ptr(v), *args, float(temperature), k, ptr(values), ptr(labels), ptr(rest), ptr(ws), n,
-                                      stream_of(scores)), "mfl_top_labels")
+    if not 1 <= k <= min(args[3], _lib.MAX_TOP_LABELS):
+        raise ValueError(f"k must be between 1 and min(C, {_lib.MAX_TOP_LABELS}), got {k} with C = {args[3]}")
+    shape, device = tuple(scores.shape), scores.device
+    values = torch.empty((shape[0], k) + shape[2:], dtype=scores.dtype, device=device)
+    labels = torch.empty((shape[0], k) + shape[2:], dtype=torch.int32, device=device)
+    rest = torch.empty((shape[0],) + shape[2:], dtype=torch.float32, device=device)
+    n = lib.mfl_top_labels_workspace_bytes(*args[2:5], args[1], k)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    _lib.call_scores(lib.mfl_top_labels, "mfl_top_labels", v, *args, temperature, k, values.data_ptr(), labels.data_ptr(),
+                     rest.data_ptr(), _address(ws), n)
     return values, labels, rest
 
 
 def _record(scores, top_scores, top_labels, rest, valid):
-    """The teacher's side of a distillation call, checked: (values, labels, rest, valid as bytes)."""
-    shape = tuple(scores.shape)
-    if top_scores.dim() != scores.dim():
-        raise RuntimeError(f"top_scores must be [N, k, ...] beside scores {shape}, got {tuple(top_scores.shape)}")
+    """The teacher's side of a distillation call, checked, as tensors to keep alive and arguments."""
+    shape = scores.shape
+    if len(top_scores.shape) != len(shape):
+        raise RuntimeError(f"top_scores must be [N, k, ...] beside scores {tuple(shape)}, got {tuple(top_scores.shape)}")
     k = top_scores.shape[1]
     if not 1 <= k <= _lib.MAX_TOP_LABELS:
         raise ValueError(f"a record holds between 1 and {_lib.MAX_TOP_LABELS} labels, got {k}")
-    rows, record = (shape[0],) + shape[2:], (shape[0], k) + shape[2:]
-    top_scores = _like_rows(scores, top_scores, "top_scores", tuple(_lib.SCORE_DTYPES), record)
-    top_labels = _like_rows(scores, top_labels, "top_labels", (torch.int32,), record)
-    rest = None if rest is None else _like_rows(scores, rest, "rest", (torch.float32,), rows)
-    valid = None if valid is None else _like_rows(scores, valid, "valid", (torch.bool, torch.uint8), rows)
-    return top_scores, top_labels, rest, valid
+    rows, record = shape[:1] + shape[2:], shape[:1] + (k,) + shape[2:]
+    top_scores = _beside(scores, top_scores, "top_scores", _lib.SCORE_DTYPES, record)
+    top_labels = _beside(scores, top_labels, "top_labels", _I32, record)
+    rest = None if rest is None else _beside(scores, rest, "rest", _F32, rows)
+    valid = None if valid is None else _beside(scores, valid, "valid", _FLAGS, rows)
+    return (top_scores, top_labels, rest, valid), (top_scores.data_ptr(), _lib.SCORE_DTYPES[top_scores.dtype], top_labels.data_ptr(),
+                                                   _address(rest), _address(valid), k), rows
+
+
+def _distillation_forward(scores, v, args, record, rows, temperature):
+    loss = torch.empty(rows, dtype=torch.float32, device=scores.device)
+    stats = torch.empty((4,) + rows, dtype=torch.float32, device=scores.device)
+    n = lib.mfl_distillation_workspace_bytes(*args[2:5], args[1], record[5])
+    ws = torch.empty(n, dtype=torch.uint8, device=scores.device) if n else None
+    _lib.call_scores(lib.mfl_distillation_forward, "mfl_distillation_forward", v, *args, *record, temperature, loss.data_ptr(),
+                     stats.data_ptr(), _address(ws), n)
+    return loss, stats
+
+
+def _distillation_backward(scores, v, args, record, stats, grad_loss, temperature):
+    grad = torch.empty_like(scores, requires_grad=False)
+    g, out = _score_rows(grad, "the gradient")
+    if out[0] != grad.data_ptr():                          # (a layout without one common stride)
+        grad = torch.empty_like(scores, memory_format=torch.contiguous_format, requires_grad=False)
+        g, out = _score_rows(grad, "the gradient")
+    _lib.call_scores(lib.mfl_distillation_backward, "mfl_distillation_backward", v, *args, *record, temperature, stats.data_ptr(),
+                     grad_loss.data_ptr(), out[0], *out[5:])
+    return grad
 
 
 def distillation_forward(scores, top_scores, top_labels, rest=None, temperature: float = 1.0, valid=None):
@@ -235,41 +271,19 @@ def distillation_forward(scores, top_scores, top_labels, rest=None, temperature:
     temperature): T^2 KL(teacher || softmax(scores / T)) over the record's labels and, with `rest`, everything else as one
     more outcome; without it the record is renormalised.  Labels outside [0, C) are passed over; rows with valid = False or
     without teacher mass have loss 0.  Returns (loss [N, ...] float32, stats for distillation_backward)."""
-    _lib.require_scores(scores)
     v, args = _score_rows(scores)
-    values, labels, rest, valid = _record(scores, top_scores, top_labels, rest, valid)
-    rows = (scores.shape[0],) + tuple(scores.shape[2:])
-    loss = torch.empty(rows, dtype=torch.float32, device=scores.device)
-    stats = torch.empty((4,) + rows, dtype=torch.float32, device=scores.device)
-    k = values.shape[1]
-    with torch.cuda.device(scores.device):
-        n = int(lib.mfl_distillation_workspace_bytes(args[1], args[2], args[3], args[0], k))
-        ws = _score_workspace(n, scores)
-        _lib.check(lib.mfl_distillation_forward(ptr(v), *args, ptr(values), _lib.SCORE_DTYPES[values.dtype], ptr(labels), ptr(rest),
-                                                ptr(valid), k, float(temperature), ptr(loss), ptr(stats), ptr(ws), n,
-                                                stream_of(scores)), "mfl_distillation_forward")
-    return loss, stats
+    _, record, rows = _record(scores, top_scores, top_labels, rest, valid)
+    return _distillation_forward(scores, v, args, record, rows, temperature)
 
 
 def distillation_backward(scores, top_scores, top_labels, stats, grad_loss, rest=None, temperature: float = 1.0, valid=None):
     """Gradient of sum(grad_loss * loss) of distillation_forward with respect to the scores, in their type and layout;
     the other arguments as there, stats as it returned them."""
-    _lib.require_scores(scores)
     v, args = _score_rows(scores)
-    values, labels, rest, valid = _record(scores, top_scores, top_labels, rest, valid)
-    rows = (scores.shape[0],) + tuple(scores.shape[2:])
-    stats = _like_rows(scores, stats, "stats", (torch.float32,), (4,) + rows)
-    grad_loss = _like_rows(scores, grad_loss, "grad_loss", (torch.float32,), rows)
-    grad = torch.empty_like(scores, requires_grad=False)
-    g, gargs = _score_rows(grad, "gradient")
-    if g.data_ptr() != grad.data_ptr():                  # (a layout without one common stride)
-        grad = torch.empty_like(scores, memory_format=torch.contiguous_format, requires_grad=False)
-        g, gargs = _score_rows(grad, "gradient")
-    with torch.cuda.device(scores.device):
-        _lib.check(lib.mfl_distillation_backward(ptr(v), *args, ptr(values), _lib.SCORE_DTYPES[values.dtype], ptr(labels), ptr(rest),
-                                                 ptr(valid), values.shape[1], float(temperature), ptr(stats), ptr(grad_loss), ptr(g),
-                                                 *gargs[4:], stream_of(scores)), "mfl_distillation_backward")
-    return grad
+    _, record, rows = _record(scores, top_scores, top_labels, rest, valid)
+    stats = _beside(scores, stats, "stats", _F32, (4,) + rows)
+    grad_loss = _beside(scores, grad_loss, "grad_loss", _F32, rows)
+    return _distillation_backward(scores, v, args, record, stats, grad_loss, temperature)
 
 
 _SAMPLE_LABEL_TYPES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
@@ -284,29 +298,26 @@ def sample_labels(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     top_k <= 0, top_p >= 1 and min_p <= 0 mean the same as 0, 0, 1 and 0.  A row without a finite largest score (all -inf,
     or a NaN or +inf in it) gets label -1 (255, the void label, with dtype=torch.uint8, which needs C <= 255).
     Returns labels [N, ...], or (labels, logprob) with the logarithm of the drawn label's share of the kept mass."""
-    _lib.require_scores(scores)
     v, args = _score_rows(scores)
-    N, rows = scores.shape[0], (scores.shape[0],) + tuple(scores.shape[2:])
-    uniform = _like_rows(scores, uniform, "uniform", (torch.float32,), rows)
+    N, rows = scores.shape[0], scores.shape[:1] + scores.shape[2:]
+    uniform = _beside(scores, uniform, "uniform", _F32, rows)
     if dtype not in _SAMPLE_LABEL_TYPES:
         raise TypeError(f"labels are uint8, int32 or int64, not {dtype}")
-    if dtype == torch.uint8 and args[2] > 255:
-        raise ValueError(f"uint8 labels hold at most 255 labels and the void one, got C = {args[2]}")
-    settings = []
-    for name, x, kind in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                          ("min_p", min_p, torch.float32)):
+    if dtype == torch.uint8 and args[3] > 255:
+        raise ValueError(f"uint8 labels hold at most 255 labels and the void one, got C = {args[3]}")
+    settings, keep = [], []
+    for name, x, kinds in (("temperature", temperature, _F32), ("top_k", top_k, _I32), ("top_p", top_p, _F32), ("min_p", min_p, _F32)):
         if torch.is_tensor(x):
-            settings += [0 if kind == torch.int32 else 0.0, _like_rows(scores, x, name, (kind,), (N,))]
+            keep.append(_beside(scores, x, name, kinds, (N,)))
+            settings += [0, keep[-1].data_ptr()]
         else:
-            settings += [int(x) if kind == torch.int32 else float(x), None]
+            settings += [x, None]
     labels = torch.empty(rows, dtype=dtype, device=scores.device)
     logprob = torch.empty(rows, dtype=torch.float32, device=scores.device) if want_logprob else None
-    with torch.cuda.device(scores.device):
-        n = int(lib.mfl_sample_labels_workspace_bytes(args[1], args[2], args[3], args[0]))
-        ws = _score_workspace(n, scores)
-        call = [ptr(x) if torch.is_tensor(x) or x is None else x for x in settings]
-        _lib.check(lib.mfl_sample_labels(ptr(v), *args, ptr(uniform), *call, ptr(labels), _SAMPLE_LABEL_TYPES[dtype], ptr(logprob),
-                                         ptr(ws), n, stream_of(scores)), "mfl_sample_labels")
+    n = lib.mfl_sample_labels_workspace_bytes(*args[2:5], args[1])
+    ws = torch.empty(n, dtype=torch.uint8, device=scores.device) if n else None
+    _lib.call_scores(lib.mfl_sample_labels, "mfl_sample_labels", v, *args, uniform.data_ptr(), *settings, labels.data_ptr(),
+                     _SAMPLE_LABEL_TYPES[dtype], _address(logprob), _address(ws), n)
     return (labels, logprob) if want_logprob else labels
 
 

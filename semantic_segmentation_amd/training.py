@@ -43,20 +43,25 @@ def per_image_nll(log_probs: torch.Tensor, labels: torch.Tensor, weight: Optiona
 
 
 class _DistillationFunction(torch.autograd.Function):
-    """Per-row distillation loss; backward by the library."""
+    """Per-row distillation loss; backward by the library (the arguments were checked on the way in)."""
 
     @staticmethod
     def forward(ctx, scores, top_scores, top_labels, rest, temperature, valid):
-        loss, stats = ops.distillation_forward(scores, top_scores, top_labels, rest, temperature, valid)
-        ctx.temperature = temperature
-        ctx.save_for_backward(scores, top_scores, top_labels, rest, valid, stats)
+        v, args = ops._score_rows(scores)
+        kept, record, rows = ops._record(scores, top_scores, top_labels, rest, valid)
+        loss, stats = ops._distillation_forward(scores, v, args, record, rows, temperature)
+        ctx.temperature, ctx.k = temperature, record[5]
+        ctx.save_for_backward(scores, *kept, stats)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
-        scores, top_scores, top_labels, rest, valid, stats = ctx.saved_tensors
-        grad = ops.distillation_backward(scores, top_scores, top_labels, stats, grad_loss, rest, ctx.temperature, valid)
+        scores, values, labels, rest, valid, stats = ctx.saved_tensors
+        v, args = ops._score_rows(scores)
+        record = (values.data_ptr(), ops._lib.SCORE_DTYPES[values.dtype], labels.data_ptr(), ops._address(rest),
+                  ops._address(valid), ctx.k)
+        grad = ops._distillation_backward(scores, v, args, record, stats, grad_loss.contiguous(), ctx.temperature)
         return grad, None, None, None, None, None
 
 
