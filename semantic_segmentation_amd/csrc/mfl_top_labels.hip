@@ -4,13 +4,13 @@
 //
 // Order: larger score first, lower label first among equals, NaN above everything.
 //
-// Two shapes of work.
+// Two shapes of work, here and in the other operators on rows.
 //   lanes   one lane per row, the k best in the lane's registers, labels streamed once.  Neighbouring pixels of a label
-//           map are neighbouring lanes, so every load of a class plane is coalesced.  A new score is sorted in
-//           (a compare, a median and two selects per place); what falls off the list's end can no longer be among the k best
-//           and goes into the rest's running sum, so one pass gives both and the rest is never a difference of two sums.
-//   rows    one workgroup per row, for rows of many labels.
-#include "mfl_scores.h"
+//           map are neighbouring lanes, so every load of a class plane is coalesced.  A new score is sorted in; what falls
+//           off the list's end can no longer be among the k best and goes into the rest's running sum, so one pass gives
+//           both and the rest is never a difference of two sums.
+//   rows    one or more waves per row, for rows of many labels (mfl_wave_top.h).
+#include "mfl_wave_top.h"
 
 namespace {
 
@@ -26,41 +26,20 @@ top_lanes_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, 
     if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    constexpr int kNone = (int)0x80000000;          // below every score's key
-    int v[K], id[K];
-#pragma unroll
-    for (int j = 0; j < K; ++j) { v[j] = kNone; id[j] = -1; }
+    Best<K> best;
     LogSum sum = {-INFINITY, 0.f};
-    // From the last place up: a place whose holder is smaller takes the new score or, where that goes further up, the holder
-    // above (strictly smaller: an earlier label stays in front of its equals).  Returns what falls off, the smallest of the
-    // K + 1.
-    auto insert = [&](float x, int c) {
-        const int xv = score_key(x);
-        const int off = min(xv, v[K - 1]);
-        bool up = xv > v[K - 1];
-#pragma unroll
-        for (int j = K - 1; j > 0; --j) {
-            const bool above = xv > v[j - 1];
-            id[j] = up ? (above ? id[j - 1] : c) : id[j];
-            v[j] = max(min(v[j - 1], xv), v[j]);    // the middle one of the three
-            up = above;
-        }
-        id[0] = up ? c : id[0];
-        v[0] = max(v[0], xv);
-        return off;
-    };
     const int head = in.C < K ? in.C : K;           // nothing real falls off before the list is full
     int c = 0;
-    for (; c < head; ++c, p += in.sc) insert(to_float(*p), c);
+    for (; c < head; ++c, p += in.sc) best.insert(place_of(to_float(*p), c));
     constexpr int U = 8;
-    for (; c + U <= in.C; c += U, p += U * in.sc) {
-        float x[U];
+    for (; c + U <= in.C; c += U) {
+        T raw[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) x[i] = to_float(p[i * in.sc]);
-        float m = sum.m;
+        for (int i = 0; i < U; ++i, p += in.sc) raw[i] = *p;
+        float x[U], m = sum.m;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            x[i] = key_score(insert(x[i], c + i));
+            x[i] = place_score(best.insert(place_of(to_float(raw[i]), c + i)));
             m = fmaxf(m, x[i]);
         }
         const float ref = finite_or_zero(m);
@@ -69,74 +48,92 @@ top_lanes_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, 
         for (int i = 0; i < U; ++i) t += __builtin_amdgcn_exp2f((x[i] - ref) * c2);
         sum = {m, t};
     }
-    for (; c < in.C; ++c, p += in.sc) add_score(sum, key_score(insert(to_float(*p), c)), c2);
+    for (; c < in.C; ++c, p += in.sc) add_score(sum, place_score(best.insert(place_of(to_float(*p), c))), c2);
     const size_t base = ((size_t)n * k) * in.S + s;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
         if (j < k) {
-            from_float(key_score(v[j]), values[base + (size_t)j * in.S]);
-            labels[base + (size_t)j * in.S] = id[j];
-        } else if (v[j] != kNone) {
-            add_score(sum, key_score(v[j]), c2);
+            from_float(place_score(best.v[j]), values[base + (size_t)j * in.S]);
+            labels[base + (size_t)j * in.S] = place_label(best.v[j]);
+        } else if (best.v[j] != 0.0) {
+            add_score(sum, place_score(best.v[j]), c2);
         }
     }
     rest[r] = log_of(sum, inv_t);
 }
 
-// One workgroup per row: k times the best label below the one before, then the rest in one pass.
+// One wave per part of a row.  With one part the row is finished here, else the part's best go to the workspace.
 template <typename T>
-__global__ void __launch_bounds__(256)
-top_rows_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
+__global__ void __launch_bounds__(kWaveTopThreads)
+top_parts_kernel(Rows in, float c2, float inv_t, int k, int parts, uint64_t *__restrict__ keys, LogSum *__restrict__ sums,
+                 T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
 {
-    __shared__ uint64_t best[4];
-    __shared__ LogSum part[4];
-    const unsigned r = blockIdx.x;
+    __shared__ uint64_t lists[kWaveTopThreads / 64][kListKeys];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned unit = blockIdx.x * (kWaveTopThreads / 64) + wave;
+    const unsigned r = unit / parts, part = unit - r * parts;
+    if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    const size_t base = ((size_t)n * k) * in.S + s;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    uint64_t last = ~0ull;
-    for (int j = 0; j < k; ++j) {
-        uint64_t b = 0;
-        for (int c = threadIdx.x; c < in.C; c += 256) {
-            const uint64_t key = rank_key(score_key(to_float(p[c * in.sc])), c);
-            if ((j == 0 || key < last) && key > b) b = key;     // (the key of a NaN on label 0 is ~0)
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)b, o);
-            b = other > b ? other : b;
-        }
-        if (lane == 0) best[wave] = b;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) b = best[w] > b ? best[w] : b;
-        __syncthreads();
-        last = b;
-        if (threadIdx.x == 0) {
-            from_float(rank_score(b), values[base + (size_t)j * in.S]);
-            labels[base + (size_t)j * in.S] = rank_label(b);
-        }
+    WaveTop<true> top(lists[wave], k, c2);
+    const int size = top_part_labels(in.C, parts);
+    const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
+    top.stream(p, in.sc, begin, end);
+    top.cut();
+    const LogSum sum = wave_join(top.rest, c2);
+    if (parts > 1) {
+        for (int j = lane; j < k; j += 64) keys[(size_t)unit * k + j] = j < top.count ? lists[wave][j] : 0;
+        if (lane == 0) sums[unit] = sum;
+        return;
     }
-    LogSum sum = {-INFINITY, 0.f};
-    for (int c = threadIdx.x; c < in.C; c += 256) {
-        const float x = to_float(p[c * in.sc]);
-        if (rank_key(score_key(x), c) < last) add_score(sum, x, c2);
-    }
-    sum = wave_join(sum, c2);
-    if (lane == 0) part[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 4; ++w) sum = join(sum, part[w], c2);
-        rest[r] = log_of(sum, inv_t);
-    }
+    const size_t base = (size_t)n * k * in.S + s;
+    top.ranked([&](int rank, uint64_t key) {
+        from_float(rank_score(key), values[base + (size_t)rank * in.S]);
+        labels[base + (size_t)rank * in.S] = rank_label(key);
+    });
+    if (lane == 0) rest[r] = log_of(sum, inv_t);
 }
 
+// One wave per row: the best of its parts' best
 template <typename T>
-int run(const Rows &in, double temperature, int k, void *values, int *labels, float *rest, hipStream_t st)
+__global__ void __launch_bounds__(64)
+top_join_kernel(Rows in, float c2, float inv_t, int k, int parts, const uint64_t *__restrict__ keys, const LogSum *__restrict__ sums,
+                T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
+{
+    __shared__ uint64_t list[kListKeys];
+    const int lane = threadIdx.x;
+    const unsigned r = blockIdx.x;
+    const unsigned n = r / in.S, s = r - n * in.S;
+    WaveTop<true> top(list, k, c2);
+    top.join(keys + (size_t)r * parts * k, parts * k);
+    top.cut();
+    for (int i = lane; i < parts; i += 64) top.rest = join(top.rest, sums[(size_t)r * parts + i], c2);
+    const LogSum sum = wave_join(top.rest, c2);
+    const size_t base = (size_t)n * k * in.S + s;
+    top.ranked([&](int rank, uint64_t key) {
+        from_float(rank_score(key), values[base + (size_t)rank * in.S]);
+        labels[base + (size_t)rank * in.S] = rank_label(key);
+    });
+    if (lane == 0) rest[r] = log_of(sum, inv_t);
+}
+
+// Rows of many neighbouring labels, long lists, and few rows go to waves
+bool by_waves(const Rows &in, int k) { return k > 32 || in.C > kBestLabels || in.rows < 64 || (in.sc == 1 && in.C >= 256); }
+
+template <typename T>
+int run(const Rows &in, double temperature, int k, void *values, int *labels, float *rest, void *workspace, hipStream_t st)
 {
     const float c2 = (float)(kLog2eD / temperature), inv_t = (float)(1.0 / temperature);
-    if (k > 32 || (in.sc == 1 && in.C >= 512) || in.rows < 64) {
-        hipLaunchKernelGGL(top_rows_kernel<T>, dim3(in.rows), dim3(256), 0, st, in, c2, inv_t, k, (T *)values, labels, rest);
+    if (by_waves(in, k)) {
+        const int parts = top_parts(in.rows, in.C);
+        uint64_t *keys = (uint64_t *)workspace;
+        LogSum *sums = (LogSum *)(keys + (size_t)in.rows * parts * k);
+        const size_t units = (size_t)in.rows * parts, per = kWaveTopThreads / 64;
+        hipLaunchKernelGGL(top_parts_kernel<T>, dim3((unsigned)((units + per - 1) / per)), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k,
+                           parts, keys, sums, (T *)values, labels, rest);
+        if (parts > 1)
+            hipLaunchKernelGGL(top_join_kernel<T>, dim3(in.rows), dim3(64), 0, st, in, c2, inv_t, k, parts, keys, sums, (T *)values, labels,
+                               rest);
         return (int)hipGetLastError();
     }
     const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
@@ -157,8 +154,10 @@ extern "C" {
 
 size_t mfl_top_labels_workspace_bytes(int N, int C, int S, int dtype, int k)
 {
-    (void)N, (void)C, (void)S, (void)dtype, (void)k;
-    return 0;
+    Rows in;
+    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || k < 1 || k > MFL_MAX_TOP_LABELS) return 0;
+    const int parts = top_parts(in.rows, in.C);
+    return parts > 1 ? (size_t)in.rows * parts * (k * sizeof(uint64_t) + sizeof(LogSum)) : 0;
 }
 
 int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c, long long stride_s,
@@ -170,13 +169,13 @@ int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long
     if (rc) return rc;
     if (!values || !labels || !rest || k < 1 || k > MFL_MAX_TOP_LABELS || k > C || !temperature_ok(temperature))
         return MFL_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < mfl_top_labels_workspace_bytes(N, C, S, dtype, k)) return MFL_ERR_WORKSPACE;
-    (void)workspace;
+    const size_t need = by_waves(in, k) ? mfl_top_labels_workspace_bytes(N, C, S, dtype, k) : 0;
+    if (need && (!workspace || workspace_bytes < need)) return MFL_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case MFL_F32: return run<float>(in, temperature, k, values, labels, rest, st);
-    case MFL_BF16: return run<bf16_t>(in, temperature, k, values, labels, rest, st);
-    default: return run<f16_t>(in, temperature, k, values, labels, rest, st);
+    case MFL_F32: return run<float>(in, temperature, k, values, labels, rest, workspace, st);
+    case MFL_BF16: return run<bf16_t>(in, temperature, k, values, labels, rest, workspace, st);
+    default: return run<f16_t>(in, temperature, k, values, labels, rest, workspace, st);
     }
 }
 
