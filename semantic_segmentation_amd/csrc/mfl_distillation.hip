@@ -227,9 +227,7 @@ __device__ inline void add_labels(const LaneRecord<T, KB, ALL> &record, const fl
     float m = out.m, y[CB];
 #pragma unroll
     for (int i = 0; i < CB; ++i) {
-        // (-inf where marked, by its bits: two instructions)
-        const int mark = (int)(marks << (31 - i)) >> 31, bits = __builtin_bit_cast(int, x[i]);
-        y[i] = __builtin_bit_cast(float, (mark & (int)0xff800000) | (~mark & bits));
+        y[i] = minus_inf_where(marks, i, x[i]);
         m = fmaxf(m, y[i]);
     }
     const float ref = finite_or_zero(m);

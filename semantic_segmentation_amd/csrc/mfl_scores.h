@@ -38,9 +38,9 @@ __device__ inline void from_float(float v, bf16_t &o) { o.u = __builtin_bit_cast
 typedef uint32_t words4 __attribute__((ext_vector_type(4)));
 typedef words4 words4_at2 __attribute__((aligned(2)));
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
-template <typename T> __device__ inline void load_vec(const T *p, float (&x)[kVec<T>])
+template <typename T> __device__ inline words4 load_words(const T *p) { return *(const words4_at2 *)p; }
+template <typename T> __device__ inline void unpack(words4 w, float (&x)[kVec<T>])
 {
-    const words4 w = *(const words4_at2 *)p;
 #pragma unroll
     for (int i = 0; i < kVec<T>; ++i) {
         // (a copy: a bit cast of a vector's element takes its first one)
@@ -49,6 +49,7 @@ template <typename T> __device__ inline void load_vec(const T *p, float (&x)[kVe
         else x[i] = to_float(__builtin_bit_cast(T, (uint16_t)(u >> (16 * (i & 1)))));
     }
 }
+template <typename T> __device__ inline void load_vec(const T *p, float (&x)[kVec<T>]) { unpack<T>(load_words(p), x); }
 template <typename T> __device__ inline void store_vec(T *p, const float (&x)[kVec<T>])
 {
     words4 w;
@@ -200,6 +201,13 @@ __device__ inline Excess wave_join(Excess a, float c)
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) a = join(a, Excess{__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, c);
     return a;
+}
+
+// -inf where bit i of the mask is set, by its bits: two instructions
+__device__ inline float minus_inf_where(uint32_t mask, int i, float x)
+{
+    const int m = (int)(mask << (31 - i)) >> 31;
+    return __builtin_bit_cast(float, (m & (int)0xff800000) | (~m & __builtin_bit_cast(int, x)));
 }
 
 // log(1 + s) for s >= -1 to a few steps: log(u) of the rounded u = 1 + s, scaled by the part of s that u keeps (Kahan)

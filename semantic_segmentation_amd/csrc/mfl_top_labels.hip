@@ -62,36 +62,63 @@ top_lanes_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, 
     rest[r] = log_of(sum, inv_t);
 }
 
-// One wave per part of a row.  With one part the row is finished here, else the part's best go to the workspace.
 template <typename T>
-__global__ void __launch_bounds__(kWaveTopThreads)
-top_parts_kernel(Rows in, float c2, float inv_t, int k, int parts, uint64_t *__restrict__ keys, LogSum *__restrict__ sums,
-                 T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
+__device__ inline void put_row(const WaveTop<true> &top, const Rows &in, unsigned r, int k, float inv_t, T *values, int *labels, float *rest)
 {
-    __shared__ uint64_t lists[kWaveTopThreads / 64][kListKeys];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned unit = blockIdx.x * (kWaveTopThreads / 64) + wave;
-    const unsigned r = unit / parts, part = unit - r * parts;
-    if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
-    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    WaveTop<true> top(lists[wave], k, c2);
-    const int size = top_part_labels(in.C, parts);
-    const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
-    top.stream(p, in.sc, begin, end);
-    top.cut();
-    const LogSum sum = wave_join(top.rest, c2);
-    if (parts > 1) {
-        for (int j = lane; j < k; j += 64) keys[(size_t)unit * k + j] = j < top.count ? lists[wave][j] : 0;
-        if (lane == 0) sums[unit] = sum;
-        return;
-    }
     const size_t base = (size_t)n * k * in.S + s;
     top.ranked([&](int rank, uint64_t key) {
         from_float(rank_score(key), values[base + (size_t)rank * in.S]);
         labels[base + (size_t)rank * in.S] = rank_label(key);
     });
-    if (lane == 0) rest[r] = log_of(sum, inv_t);
+    const LogSum sum = wave_join(top.rest, top.c2);
+    if ((threadIdx.x & 63) == 0) rest[r] = log_of(sum, inv_t);
+}
+
+// One wave per row
+template <typename T>
+__global__ void __launch_bounds__(kWaveTopThreads)
+top_waves_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
+{
+    __shared__ uint64_t lists[kWaveTopThreads / 64][kListKeys];
+    const int wave = threadIdx.x >> 6;
+    const unsigned r = blockIdx.x * (kWaveTopThreads / 64) + wave;
+    if (r >= in.rows) return;
+    const unsigned n = r / in.S, s = r - n * in.S;
+    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
+    WaveTop<true> top(lists[wave], k, c2);
+    if (in.sc == 1 && in.C >= 8 * 64 * kVec<T>) {
+        float m[4];
+        top.look(p, 0, 4, m);
+        top.foresee(m);
+    }
+    top.stream(p, in.sc, 0, in.C);
+    top.cut();
+    put_row(top, in, r, k, inv_t, values, labels, rest);
+}
+
+// One workgroup per part of a row.  With one part the row is finished here, else the part's best go to the workspace.
+template <typename T>
+__global__ void __launch_bounds__(kWaveTopThreads)
+top_parts_kernel(Rows in, float c2, float inv_t, int k, int parts, uint64_t *__restrict__ keys, LogSum *__restrict__ sums,
+                 T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
+{
+    __shared__ TopShared sh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const unsigned n = r / in.S, s = r - n * in.S;
+    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
+    WaveTop<true> top(sh.lists[wave], k, c2);
+    const int size = top_part_labels(in.C, parts);
+    const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
+    if (!top_of_part(top, sh, p, in.sc, begin, end)) return;
+    if (parts == 1) {
+        put_row(top, in, r, k, inv_t, values, labels, rest);
+        return;
+    }
+    for (int j = lane; j < k; j += 64) keys[(size_t)blockIdx.x * k + j] = j < top.count ? top.list[j] : 0;
+    const LogSum sum = wave_join(top.rest, c2);
+    if (lane == 0) sums[blockIdx.x] = sum;
 }
 
 // One wave per row: the best of its parts' best
@@ -103,18 +130,11 @@ top_join_kernel(Rows in, float c2, float inv_t, int k, int parts, const uint64_t
     __shared__ uint64_t list[kListKeys];
     const int lane = threadIdx.x;
     const unsigned r = blockIdx.x;
-    const unsigned n = r / in.S, s = r - n * in.S;
     WaveTop<true> top(list, k, c2);
     top.join(keys + (size_t)r * parts * k, parts * k);
     top.cut();
     for (int i = lane; i < parts; i += 64) top.rest = join(top.rest, sums[(size_t)r * parts + i], c2);
-    const LogSum sum = wave_join(top.rest, c2);
-    const size_t base = (size_t)n * k * in.S + s;
-    top.ranked([&](int rank, uint64_t key) {
-        from_float(rank_score(key), values[base + (size_t)rank * in.S]);
-        labels[base + (size_t)rank * in.S] = rank_label(key);
-    });
-    if (lane == 0) rest[r] = log_of(sum, inv_t);
+    put_row(top, in, r, k, inv_t, values, labels, rest);
 }
 
 // Rows of many neighbouring labels, long lists, and few rows go to waves
@@ -125,12 +145,17 @@ int run(const Rows &in, double temperature, int k, void *values, int *labels, fl
 {
     const float c2 = (float)(kLog2eD / temperature), inv_t = (float)(1.0 / temperature);
     if (by_waves(in, k)) {
+        if (in.C < kBlockLabels) {
+            const unsigned per = kWaveTopThreads / 64;
+            hipLaunchKernelGGL(top_waves_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k,
+                               (T *)values, labels, rest);
+            return (int)hipGetLastError();
+        }
         const int parts = top_parts(in.rows, in.C);
         uint64_t *keys = (uint64_t *)workspace;
         LogSum *sums = (LogSum *)(keys + (size_t)in.rows * parts * k);
-        const size_t units = (size_t)in.rows * parts, per = kWaveTopThreads / 64;
-        hipLaunchKernelGGL(top_parts_kernel<T>, dim3((unsigned)((units + per - 1) / per)), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k,
-                           parts, keys, sums, (T *)values, labels, rest);
+        hipLaunchKernelGGL(top_parts_kernel<T>, dim3(in.rows * parts), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k, parts, keys, sums,
+                           (T *)values, labels, rest);
         if (parts > 1)
             hipLaunchKernelGGL(top_join_kernel<T>, dim3(in.rows), dim3(64), 0, st, in, c2, inv_t, k, parts, keys, sums, (T *)values, labels,
                                rest);

@@ -1,10 +1,11 @@
 // The k <= 128 largest scores of a run of labels, by one wave in one pass (mfl_top_labels.hip, mfl_sample_labels.hip).
 //
 // The wave keeps a list of candidates in LDS, as rank keys, and a bound below which no label can be among the k best any
-// more.  A vector of scores with none above the bound costs a maximum and a compare; scores above it are appended.  When
-// the list is full, a binary search over the keys (held in registers, eight a lane, counted by ballots) finds a bound that
-// leaves between k and about 2 k of them, and the others leave.  For scores in random order about k ln(C / 512) of C labels
-// are appended at all; for rising ones every label is, at one search per few hundred.  Everything that never enters or
+// more.  A vector of scores with none above the bound costs a compare each; scores above it are appended.  When
+// the list has grown, a binary search over the keys (held in registers, counted by ballots) finds a bound that
+// leaves between k and about 2 k of them, and the others leave.  Before the first search a look at the first part's largest
+// score per lane gives a bound.  For scores in random order a few hundred labels are appended at all; for rising ones every
+// label is, at one search per few hundred.  Everything that never enters or
 // leaves the list goes into the rest's running sum exactly once.  Appending follows the order of the labels and every count
 // is the wave's own: no atomics, the same result every time.
 #ifndef MFL_WAVE_TOP_H
@@ -15,11 +16,12 @@
 namespace mfl_scores {
 
 constexpr int kWaveTopThreads = 256;
-constexpr int kListKeys = 512;
-constexpr int kListRegs = kListKeys / 64;
+constexpr int kListKeys = 1024;
+
+typedef __attribute__((address_space(3))) uint64_t lds_key;
 
 template <bool REST> struct WaveTop {
-    uint64_t *list;             // LDS, kListKeys, this wave's own
+    lds_key *list;              // kListKeys, this wave's own
     int k, count;
     uint64_t bound;             // keys up to it are out
     float bound_score;
@@ -27,82 +29,181 @@ template <bool REST> struct WaveTop {
     LogSum rest;                // this lane's share
 
     __device__ WaveTop(uint64_t *list, int k, float c2)
-        : list(list), k(k), count(0), bound(0), bound_score(-INFINITY), c2(c2), rest{-INFINITY, 0.f} {}
+        : list((lds_key *)list), k(k), count(0), bound(0), bound_score(-INFINITY), c2(c2), rest{-INFINITY, 0.f} {}
 
     // Leaves between `least` (<= count) and `most` keys in the list
     __device__ void shrink(int least, int most)
     {
+        constexpr int R = kListKeys / 128;          // registers of half a list
         const int lane = threadIdx.x & 63;
-        uint64_t r[kListRegs];
+        const bool both = count > kListKeys / 2;    // the second half holds something
+        uint64_t r[2][R];
         __builtin_amdgcn_wave_barrier();
+        auto load = [&](uint64_t (&h)[R], int from) {
 #pragma unroll
-        for (int i = 0; i < kListRegs; ++i) r[i] = lane + 64 * i < count ? list[lane + 64 * i] : 0;
-        uint64_t lo = bound, hi = ~0ull;            // more than `most` above lo, fewer than `least` above hi
-        uint64_t mid;
-        for (;;) {
-            mid = lo + (hi - lo) / 2;               // (keys differ: least = most is always met)
-            int above = 0;
+            for (int i = 0; i < R; ++i) h[i] = from + 64 * i + lane < count ? list[from + 64 * i + lane] : 0;
+        };
+        load(r[0], 0);
+        if (both) load(r[1], kListKeys / 2);
+        auto scores_above = [&](const uint64_t (&h)[R], uint32_t at) {
+            int n = 0;
 #pragma unroll
-            for (int i = 0; i < kListRegs; ++i) above += __popcll(__ballot(r[i] > mid));
-            if (above > most) lo = mid;
-            else if (above < least) hi = mid;
-            else break;
-            if (hi - lo <= 1) {                     // (the key ~0, a NaN on label 0, is above nothing: keep from it on)
-                mid = lo;
+            for (int i = 0; i < R; ++i) n += __popcll(__ballot((uint32_t)(h[i] >> 32) > at));
+            return n;
+        };
+        auto keys_above = [&](const uint64_t (&h)[R], uint64_t at) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < R; ++i) n += __popcll(__ballot(h[i] > at));
+            return n;
+        };
+        // by the scores first: more than `most` above lo, fewer than `least` above hi
+        uint32_t lo = (uint32_t)(bound >> 32), hi = ~0u, at = lo;
+        bool found = false;
+        while (hi - lo > 1) {
+            at = lo + (hi - lo) / 2;
+            int above = scores_above(r[0], at);
+            if (both) above += scores_above(r[1], at);
+            if (above > most) {
+                lo = at;
+            } else if (above < least) {
+                hi = at;
+            } else {
+                found = true;
                 break;
             }
         }
-        count = 0;
-#pragma unroll
-        for (int i = 0; i < kListRegs; ++i) {
-            const bool stay = r[i] > mid;
-            const uint64_t who = __ballot(stay);
-            if (stay) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = r[i];
-            count += __popcll(who);
-            if (REST && !stay && r[i]) add_score(rest, rank_score(r[i]), c2);
+        if (found) {
+            bound = (uint64_t)at << 32 | 0xffffffffu;
+        } else {
+            // too many share one score: by their labels (the scores up to lo are out, those above hi are in)
+            uint64_t mid = lo == (uint32_t)(bound >> 32) ? bound : (uint64_t)lo << 32 | 0xffffffffu;
+            uint64_t end = (uint64_t)hi << 32 | 0xffffffffu;
+            while (end - mid > 1) {
+                const uint64_t m = mid + (end - mid) / 2;
+                int above = keys_above(r[0], m);
+                if (both) above += keys_above(r[1], m);
+                if (above < least) {
+                    end = m;
+                } else {
+                    mid = m;
+                    if (above <= most) break;
+                }
+            }
+            bound = mid;
         }
-        bound = mid;
-        bound_score = rank_score(mid);
+        count = 0;
+        auto keep = [&](const uint64_t (&h)[R]) {
+            float out[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const bool stay = h[i] > bound;
+                const uint64_t who = __ballot(stay);
+                if (stay) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = h[i];
+                count += __popcll(who);
+                out[i] = stay || !h[i] ? -INFINITY : rank_score(h[i]);
+            }
+            if (REST) add_to_rest(out);
+        };
+        keep(r[0]);
+        if (both) keep(r[1]);
+        bound_score = rank_score(bound);
         __builtin_amdgcn_wave_barrier();
     }
     __device__ int most() const { return k < 64 ? 2 * k + 32 : k + k / 2; }
 
-    // Appends the keys of the lanes that bring one; returns whether this lane's went in
+    // Keeps the list short: its bound is only as tight as the last search
+    __device__ void room()
+    {
+        if (count >= most() + 128) shrink(k, most());
+    }
+    // Appends this lane's key if it brings one; returns whether it went in
     __device__ bool append(uint64_t key, bool bring)
     {
         bring = bring && key > bound;
-        uint64_t who = __ballot(bring);
-        if (!who) return false;
-        if (count + __popcll(who) > kListKeys) {
-            shrink(k, most());
-            bring = bring && key > bound;
-            who = __ballot(bring);
-        }
+        const uint64_t who = __ballot(bring);
         if (bring) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
         count += __popcll(who);
         return bring;
     }
+    template <int V> __device__ void add_to_rest(const float (&x)[V])
+    {
+        float top = rest.m;
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
+        const float ref = finite_or_zero(top);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * c2);
+        rest = {top, fmaf(rest.s, __builtin_amdgcn_exp2f((rest.m - ref) * c2), sum)};
+    }
 
     template <int V> __device__ void take(float (&x)[V], int c, int end)
     {
-        float m = x[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) m = max_or_nan(m, x[i]);
+        static_assert(MFL_MAX_TOP_LABELS * 3 / 2 + 128 + 64 * V <= kListKeys, "a vector fits behind a list that room() leaves");
+        room();
         // (a NaN is not below the bound either)
-        if (__any(!(m < bound_score))) {
+        uint32_t open = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (append(rank_key(score_key(x[i]), c + i), c + i < end)) x[i] = -INFINITY;
+        for (int i = 0; i < V; ++i) open |= !(x[i] < bound_score) ? 1u << i : 0u;
+        if (c + V > end) open &= (1u << max(end - c, 0)) - 1;
+        // every lane brings its first open score, then its second: a turn or two once the bound is tight
+        uint32_t in = 0;
+        while (__any(open != 0)) {
+            const int i = __ffs(open) - 1;
+            float v = x[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) v = i == j ? x[j] : v;
+            if (append(rank_key(score_key(v), c + i), open != 0)) in |= 1u << i;
+            open &= open - 1;
         }
         if (REST) {
-            float top = rest.m;
 #pragma unroll
-            for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
-            const float ref = finite_or_zero(top);
-            float sum = 0.f;
+            for (int j = 0; j < V; ++j) x[j] = minus_inf_where(in, j, x[j]);
+            add_to_rest(x);
+        }
+    }
+
+    // The largest scores of four disjoint sets a lane, among the first `vectors` of the labels at p + begin
+    template <typename T> __device__ static void look(const T *p, int begin, int vectors, float (&m)[4])
+    {
+        constexpr int V = kVec<T>;
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * c2);
-            rest = {top, fmaf(rest.s, __builtin_amdgcn_exp2f((rest.m - ref) * c2), sum)};
+        for (int u = 0; u < 4; ++u) m[u] = -INFINITY;
+        for (int v = 0; v < vectors; v += 4) {
+            float x[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_vec(p + begin + ((v + u) * 64 + lane) * V, x[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < V; ++i) m[u] = fmaxf(m[u], x[u][i]);
+        }
+    }
+    // A bound to begin with, from the largest scores of 256 disjoint sets of labels, four a lane: where k sets hold a score
+    // that large, k labels do.
+    __device__ void foresee(const float (&m)[4])
+    {
+        uint32_t seen[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) seen[u] = (uint32_t)score_key(m[u]) ^ 0x80000000u;
+        uint32_t lo = 0, hi = ~0u;                  // at least k sets reach lo, fewer hi
+        while (hi - lo > 1) {
+            const uint32_t at = lo + (hi - lo) / 2;
+            int n = 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) n += __popcll(__ballot(seen[u] >= at));
+            if (n >= k) {
+                lo = at;
+                if (n == k) break;
+            } else {
+                hi = at;
+            }
+        }
+        if (lo) {
+            bound = ((uint64_t)lo << 32) - 1;
+            bound_score = key_score((int)(lo ^ 0x80000000u));
         }
     }
 
@@ -112,27 +213,32 @@ template <bool REST> struct WaveTop {
         constexpr int V = kVec<T>;
         const int lane = threadIdx.x & 63;
         if (sc == 1) {
-            constexpr int U = 4;                    // vectors in flight
-            int c = begin;
-            for (; c + U * 64 * V <= end; c += U * 64 * V) {
-                float x[U][V];
-#pragma unroll
-                for (int u = 0; u < U; ++u) load_vec(p + c + (u * 64 + lane) * V, x[u]);
-#pragma unroll
-                for (int u = 0; u < U; ++u) take(x[u], c + (u * 64 + lane) * V, end);
-            }
-            for (; c < end; c += 64 * V) {
-                const int at = c + lane * V;
-                float x[V];
-                if (at + V <= end) {
-                    load_vec(p + at, x);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) x[i] = at + i < end ? to_float(p[at + i]) : -INFINITY;
+            // (one copy of the loop's body: three vectors ahead, kept as bits)
+            constexpr int step = 64 * V;
+            const int whole = begin + (end - begin) / step * step;
+            if (begin < whole) {
+                // (past the last one: the last one again, so that the count of loads in flight is the same all the way)
+                auto ahead = [&](int c) { return load_words(p + min(c, whole - step) + lane * V); };
+                words4 a = ahead(begin), b = ahead(begin + step), d = ahead(begin + 2 * step);
+#pragma unroll 1
+                for (int c = begin; c < whole; c += step) {
+                    float x[V];
+                    unpack<T>(a, x);
+                    a = b;
+                    b = d;
+                    d = ahead(c + 3 * step);
+                    take(x, c + lane * V, end);
                 }
+            }
+            if (whole < end) {
+                const int at = whole + lane * V;
+                float x[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = at + i < end ? to_float(p[at + i]) : -INFINITY;
                 take(x, at, end);
             }
         } else {
+#pragma unroll 1
             for (int c = begin; c < end; c += 64) {
                 float x[1] = {c + lane < end ? to_float(p[(c + lane) * sc]) : -INFINITY};
                 take(x, c + lane, end);
@@ -141,11 +247,13 @@ template <bool REST> struct WaveTop {
     }
 
     // Keys that other waves found (0: none)
-    __device__ void join(const uint64_t *keys, int n)
+    template <typename Key> __device__ void join(Key *keys, int n)
     {
         const int lane = threadIdx.x & 63;
+#pragma unroll 1
         for (int i = 0; i < n; i += 64) {
             const uint64_t key = i + lane < n ? keys[i + lane] : 0;
+            room();
             const bool in = append(key, key != 0);
             if (REST && !in && key) add_score(rest, rank_score(key), c2);
         }
@@ -174,11 +282,63 @@ template <bool REST> struct WaveTop {
     }
 };
 
-// Parts a row is cut into: enough waves for the card (16 on each of 256 CUs), at least 2048 labels each
+// ---- a workgroup's four waves on one part of a row, or on four rows
+//
+// Four waves on one part agree on the bound to begin with: each brings the largest scores of 64 sets of 64 labels or so, and
+// with k = 64 of 256 sets the bound lets 0.5 % of scores in random order through, an eighth of what a wave's own look at
+// 16 labels a set would.  The first wave then joins the four lists.
+
+struct TopShared {
+    uint64_t lists[kWaveTopThreads / 64][kListKeys];
+    float seen[kWaveTopThreads];
+    LogSum rest[kWaveTopThreads / 64];
+    int count[kWaveTopThreads / 64];
+};
+
+// After it the first wave's list holds the part's k best and its lanes the shares of the rest; the other waves are done.
+template <bool REST, typename T>
+__device__ inline bool top_of_part(WaveTop<REST> &top, TopShared &sh, const T *p, long long sc, int begin, int end)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int step = 64 * kVec<T>;
+    const int quarter = ((end - begin + 3) / 4 + step - 1) / step * step;
+    const int from = min(end, begin + wave * quarter), to = min(end, from + quarter);
+    // (every wave has the vectors to look at, and they are at most half of what there is)
+    const int vectors = sc == 1 && end - begin - 3 * quarter >= 8 * step ? (quarter >= 16 * step ? 8 : 4) : 0;
+    if (vectors) {
+        float m[4];
+        WaveTop<REST>::look(p, from, vectors, m);
+        sh.seen[threadIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) m[u] = sh.seen[lane + 64 * u];
+        top.foresee(m);
+    }
+    top.stream(p, sc, from, to);
+    if (top.count > kListKeys / 2) top.shrink(top.k, top.most());
+    const LogSum rest = wave_join(top.rest, top.c2);
+    if (lane == 0) {
+        sh.count[wave] = top.count;
+        sh.rest[wave] = rest;
+    }
+    __syncthreads();
+    if (wave) return false;
+    for (int w = 1; w < kWaveTopThreads / 64; ++w) {
+        top.join((lds_key *)sh.lists[w], sh.count[w]);
+        if (REST && lane == 0) top.rest = join(top.rest, sh.rest[w], top.c2);
+    }
+    top.cut();
+    return true;
+}
+
+// Labels from which on a part gets a whole workgroup
+constexpr int kBlockLabels = 8192;
+
+// Parts a row is cut into: enough workgroups for the card, at least kBlockLabels labels each
 __host__ __device__ inline int top_part_labels(int C, int parts) { return (((C + parts - 1) / parts) + 511) & ~511; }
 inline int top_parts(unsigned rows, int C)
 {
-    const unsigned most = (unsigned)((C + 2047) / 2048), want = (4096 + rows - 1) / rows;
+    const unsigned most = (unsigned)(C / kBlockLabels), want = (1024 + rows - 1) / rows;
     const unsigned n = want < most ? want : most;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
