@@ -12,12 +12,17 @@
 // sums (10^-7) would misplace about one draw in a hundred, and a batch of maps has millions of draws.
 //
 // Settings may differ from n to n (arrays of N).  T <= 0 takes the largest; top_k <= 0, top_p >= 1 and min_p <= 0 keep all.
+// Shapes of work: one lane per row (label maps), one wave or workgroup per row where top_k cuts the row to a short list
+// (mfl_wave_top.h), and one workgroup per row otherwise, which finds the cut by a histogram of the weights.
+//
 // A row without a finite largest score (all -inf, or a NaN or +inf among them) has no distribution: label -1, logprob -inf.
-#include "mfl_scores.h"
+#include "mfl_wave_top.h"
 
 namespace {
 
 using namespace mfl_scores;
+
+typedef __attribute__((address_space(3))) double lds_double;
 
 struct Settings {
     double t, top_p, min_p;
@@ -28,7 +33,6 @@ struct Settings {
 struct Filter {
     double inv_t, top_p, min_p;
     int top_k;                  // INT_MAX: no limit
-    bool ranked;                // the order of the labels matters
 };
 __device__ inline Filter filter_of(const Settings &f, unsigned n, int C)
 {
@@ -41,7 +45,8 @@ __device__ inline Filter filter_of(const Settings &f, unsigned n, int C)
     if (!(t > 0)) r.top_k = 1;
     r.inv_t = t > 0 ? fmax(1.0 / t, 1e-30) : 1.0;       // (never 0: -inf * 0)
     if (!(r.top_p < 1)) r.top_p = 1;
-    r.ranked = r.top_k < C || r.top_p < 1;
+    if (!(r.min_p > 0)) r.min_p = 0;
+    if (r.min_p > 1) r.top_k = 1, r.min_p = 0;
     return r;
 }
 
@@ -76,9 +81,9 @@ sample_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Ou
     for (int c = 0; c < in.C; ++c) mk = max(mk, score_key(to_float(p[c * in.sc])));
     const float m = key_score(mk);
     if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
-    auto weight = [&](float x) { return exp(((double)x - (double)m) * f.inv_t); };
+    const Weight weight = {m, f.inv_t * kLog2eD};
     uint64_t cut = 0;                               // kept by rank: rank_key >= cut
-    if (f.ranked) {
+    if (f.top_k < in.C || f.top_p < 1) {
         // binary search over the rank keys, from the top bit down
         auto search = [&](auto reached) {
             uint64_t k = 0;
@@ -133,9 +138,168 @@ sample_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Ou
     put(out, r, label, log(got / total));
 }
 
-// One workgroup per row.
-constexpr int kRowThreads = 256;
-template <typename V> __device__ inline V block_sum(V v, V *part)
+
+// ---- rows that top_k cuts to a short list
+
+// One wave: draws from the list (at most 128 keys, in any order) of the row's best labels
+template <bool REST>
+__device__ inline void draw_from_list(const WaveTop<REST> &top, const Filter &f, float u, unsigned r, const Out &out, lds_double *share)
+{
+    const int lane = threadIdx.x & 63;
+    uint64_t key[2], best = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        key[h] = lane + 64 * h < top.count ? top.list[lane + 64 * h] : 0;
+        best = key[h] > best ? key[h] : best;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t other = __shfl_xor((unsigned long long)best, o);
+        best = other > best ? other : best;
+    }
+    const float m = rank_score(best);
+    if (!(fabsf(m) < INFINITY)) {
+        if (lane == 0) put(out, r, -1, -INFINITY);
+        return;
+    }
+    const Weight weight = {m, f.inv_t * kLog2eD};
+    double w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w[h] = key[h] ? weight(rank_score(key[h])) : 0.0;
+        share[lane + 64 * h] = w[h];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (f.top_p < 1 || f.min_p > 0 || f.top_k < top.count) {
+        double front[2] = {0, 0}, total = 0;
+        int above[2] = {0, 0};
+        for (int j = 0; j < top.count; ++j) {
+            const uint64_t other = top.list[j];
+            const double v = share[j];
+            total += v;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                front[h] += other > key[h] ? v : 0.0;
+                above[h] += other > key[h];
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool keep = key[h] == best || (above[h] < f.top_k && (front[h] < f.top_p * total || f.top_p >= 1) && w[h] >= f.min_p);
+            w[h] = keep ? w[h] : 0.0;
+            share[lane + 64 * h] = w[h];
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    // running sums in label order
+    double upto[2] = {0, 0}, total = 0;
+    for (int j = 0; j < top.count; ++j) {
+        const int other = rank_label(top.list[j]);
+        const double v = share[j];
+        total += v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) upto[h] += other <= rank_label(key[h]) ? v : 0.0;
+    }
+    const double target = draw_of(u) * total;
+    int hit = 0x7fffffff, last = -1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (w[h] > 0) {
+            if (upto[h] > target) hit = min(hit, rank_label(key[h]));
+            last = max(last, rank_label(key[h]));
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        hit = min(hit, __shfl_xor(hit, o));
+        last = max(last, __shfl_xor(last, o));
+    }
+    const int label = hit == 0x7fffffff ? last : hit;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (key[h] && rank_label(key[h]) == label) put(out, r, label, log(w[h] / total));
+}
+
+template <typename T> struct RowOf {
+    const T *p;
+    unsigned n;
+    __device__ RowOf(const Rows &in, unsigned r)
+    {
+        n = r / in.S;
+        p = (const T *)in.p + (long long)n * in.sn + (long long)(r - n * in.S) * in.ss;
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kWaveTopThreads)
+list_waves_kernel(Rows in, Settings set, int k, const float *__restrict__ uniform, Out out)
+{
+    __shared__ uint64_t lists[kWaveTopThreads / 64][kListKeys];
+    __shared__ double share[kWaveTopThreads / 64][MFL_MAX_TOP_LABELS];
+    const int wave = threadIdx.x >> 6;
+    const unsigned r = blockIdx.x * (kWaveTopThreads / 64) + wave;
+    if (r >= in.rows) return;
+    const RowOf<T> row(in, r);
+    WaveTop<false> top(lists[wave], k, 0.f);
+    if (in.sc == 1 && in.C >= 8 * 64 * kVec<T>) {
+        float m[4];
+        top.look(row.p, 0, 4, m);
+        top.foresee(m);
+    }
+    top.stream(row.p, in.sc, 0, in.C);
+    top.cut();
+    draw_from_list(top, filter_of(set, row.n, in.C), uniform[r], r, out, (lds_double *)share[wave]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWaveTopThreads)
+list_parts_kernel(Rows in, Settings set, int k, int parts, const float *__restrict__ uniform, uint64_t *__restrict__ keys, Out out)
+{
+    __shared__ TopShared sh;
+    __shared__ double share[MFL_MAX_TOP_LABELS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const RowOf<T> row(in, r);
+    WaveTop<false> top(sh.lists[wave], k, 0.f);
+    const int size = top_part_labels(in.C, parts);
+    const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
+    if (!top_of_part(top, sh, row.p, in.sc, begin, end)) return;
+    if (parts == 1) return draw_from_list(top, filter_of(set, row.n, in.C), uniform[r], r, out, (lds_double *)share);
+    for (int j = lane; j < k; j += 64) keys[(size_t)blockIdx.x * k + j] = j < top.count ? top.list[j] : 0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(64)
+list_join_kernel(Rows in, Settings set, int k, int parts, const float *__restrict__ uniform, const uint64_t *__restrict__ keys, Out out)
+{
+    __shared__ uint64_t list[kListKeys];
+    __shared__ double share[MFL_MAX_TOP_LABELS];
+    const unsigned r = blockIdx.x;
+    WaveTop<false> top(list, k, 0.f);
+    top.join(keys + (size_t)r * parts * k, parts * k);
+    top.cut();
+    draw_from_list(top, filter_of(set, r / in.S, in.C), uniform[r], r, out, (lds_double *)share);
+}
+
+// ---- rows of many labels, any settings: one workgroup per row
+//
+//   1  the largest score
+//   2  where top_k or top_p cut: a histogram over 2048 bins of (largest - score) / T, 32 a unit: counts, and masses as
+//      64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose sums do not depend on the
+//      order of the atomics; running sums over the bins name the bin that the cut falls into
+//   3  that bin's labels, a list in LDS; every one counts what lies above it in the list, and the lowest that stays is the
+//      cut.  (A bin of more labels than the list holds, all of nearly one score: a binary search over the rank keys.)
+//   4  the kept weights summed in runs of neighbouring labels, the run that the draw falls into, the label in it
+//
+// Steps 2 to 4 read the row again, from the caches if it fits.  Weights below the cut cost a compare in step 4.
+
+constexpr int kBins = 2048;
+constexpr float kBinsPerUnit = 32.f;
+constexpr int kRuns = 1024;
+constexpr int kBinList = 2048;
+
+template <typename V, int NT> __device__ inline V block_sum(V v, V *part)
 {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -143,115 +307,370 @@ template <typename V> __device__ inline V block_sum(V v, V *part)
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = part[0];
-    for (int w = 1; w < kRowThreads / 64; ++w) v += part[w];
+    for (int w = 1; w < NT / 64; ++w) v += part[w];
     return v;
 }
-
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads)
-sample_rows_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+// Sum over the threads in front, and over all
+template <typename V, int NT> __device__ inline V block_front(V v, V *part, V &all)
 {
-    __shared__ double part[kRowThreads / 64], sums[kRowThreads];
-    __shared__ int ipart[kRowThreads / 64];
-    const unsigned r = blockIdx.x;
-    const unsigned n = r / in.S, s = r - n * in.S;
-    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    const Filter f = filter_of(set, n, in.C);
-    int mk = (int)0x80000000;
-    for (int c = threadIdx.x; c < in.C; c += kRowThreads) mk = max(mk, score_key(to_float(p[c * in.sc])));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    V upto = v;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mk = max(mk, __shfl_xor(mk, o));
-    if ((threadIdx.x & 63) == 0) ipart[threadIdx.x >> 6] = mk;
+    for (int o = 1; o < 64; o <<= 1) {
+        const V other = __shfl_up(upto, o);
+        if (lane >= o) upto += other;
+    }
     __syncthreads();
-    for (int w = 0; w < kRowThreads / 64; ++w) mk = max(mk, ipart[w]);
-    const float m = key_score(mk);
-    if (!(fabsf(m) < INFINITY)) {
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    V before = 0;
+    all = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w == wave) before = all;
+        all += part[w];
+    }
+    const V ahead = __shfl_up(upto, 1);
+    return before + (lane ? ahead : V(0));
+}
+
+template <typename T, int NT> struct BlockRow {
+    struct Shared {
+        uint32_t counts[kBins];
+        unsigned long long masses[kBins];
+        unsigned long long key[kBinList], key_mass[kBinList];
+        double runs[kRuns];
+        unsigned long long upart[NT / 64];
+        double dpart[NT / 64];
+        float fpart[NT / 64];
+        unsigned listed, bin;
+        unsigned long long bin_front, low_key;
+    };
+    Shared &sh;
+    const T *p;
+    long long sc;
+    int C;
+    float m, scale;
+    Weight weight;
+    int bits;                   // of the fixed-point masses
+
+    __device__ int bin_of(float x) const { return min((int)((m - x) * scale), kBins - 1); }
+    __device__ uint64_t mass(float x) const
+    {
+        // 2^52 + an integer below 2^52: the low bits of the sum are that integer
+        const double v = __builtin_ldexp(weight(x), bits) + 4503599627370496.0;
+        return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
+    }
+    // f(score, label) over the row
+    template <typename F> __device__ void each(F f) const
+    {
+        if (sc == 1) {
+            constexpr int V = kVec<T>, U = 2;
+            int c = threadIdx.x * V;
+            for (; c + (U - 1) * NT * V + V <= C; c += U * NT * V) {
+                float x[U][V];
+#pragma unroll
+                for (int u = 0; u < U; ++u) load_vec(p + c + u * NT * V, x[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f(x[u][i], c + u * NT * V + i);
+            }
+            for (; c < C; c += NT * V) {
+                if (c + V <= C) {
+                    float x[V];
+                    load_vec(p + c, x);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f(x[i], c + i);
+                } else {
+                    for (int i = c; i < C; ++i) f(to_float(p[i]), i);
+                }
+            }
+        } else {
+            for (int c = threadIdx.x; c < C; c += NT) f(to_float(p[c * sc]), c);
+        }
+    }
+
+    __device__ void largest()
+    {
+        float v = -INFINITY;
+        each([&](float x, int) { v = max_or_nan(v, x); });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v = max_or_nan(v, __shfl_xor(v, o));
+        if ((threadIdx.x & 63) == 0) sh.fpart[threadIdx.x >> 6] = v;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; ++w) v = max_or_nan(v, sh.fpart[w]);
+        m = v;
+    }
+
+    // The lowest rank key that stays, where labels of at least `low` stay while front < goal, front = what the labels above
+    // hold: their number (COUNT) or mass.  The sum over everything is at least goal.
+    template <bool COUNT> __device__ uint64_t cut_at(double goal, uint64_t low)
+    {
+        // the bin it falls into, and what the bins in front of it hold
+        constexpr int per = kBins / NT;
+        unsigned long long mine = 0, all;
+        for (int i = 0; i < per; ++i) mine += COUNT ? sh.counts[threadIdx.x * per + i] : sh.masses[threadIdx.x * per + i];
+        unsigned long long front = block_front<unsigned long long, NT>(mine, sh.upart, all);
+        if (threadIdx.x == 0) sh.listed = 0, sh.low_key = ~0ull;
+        if ((double)front < goal && (double)(front + mine) >= goal) {
+            int b = threadIdx.x * per;
+            for (;; ++b) {
+                const unsigned long long here = COUNT ? sh.counts[b] : sh.masses[b];
+                if ((double)(front + here) >= goal) break;
+                front += here;
+            }
+            sh.bin = b;
+            sh.bin_front = front;
+        }
+        __syncthreads();
+        const int bin = sh.bin;
+        front = sh.bin_front;
+        each([&](float x, int c) {
+            if (bin_of(x) != bin) return;
+            const uint64_t key = rank_key(score_key(x), c);
+            if (key < low) return;
+            const unsigned at = atomicAdd(&sh.listed, 1u);
+            if (at >= (unsigned)kBinList) return;
+            sh.key[at] = key;
+            sh.key_mass[at] = COUNT ? 1 : mass(x);
+        });
+        __syncthreads();
+        const int n = sh.listed;
+        if (n <= kBinList) {
+            for (int i = threadIdx.x; i < n; i += NT) {
+                const uint64_t key = sh.key[i];
+                unsigned long long above = 0;
+                for (int j = 0; j < n; ++j) above += sh.key[j] > key ? sh.key_mass[j] : 0;
+                if ((double)(front + above) < goal) atomicMin(&sh.low_key, key);
+            }
+            __syncthreads();
+            return sh.low_key;
+        }
+        // the largest key from which on at least `goal` is held
+        uint64_t best = 0;
+        for (int b = 63; b >= 0; --b) {
+            const uint64_t at = best | 1ull << b, from = at > low ? at : low;
+            unsigned long long held = 0;
+            each([&](float x, int c) {
+                if (bin_of(x) == bin && rank_key(score_key(x), c) >= from) held += COUNT ? 1 : mass(x);
+            });
+            held = block_sum<unsigned long long, NT>(held, sh.upart);
+            if ((double)(front + held) >= goal) best = at;
+        }
+        return best > low ? best : low;
+    }
+
+    // The lowest rank key that top_k and top_p keep
+    __device__ uint64_t cut(const Filter &f)
+    {
+        for (int i = threadIdx.x; i < kBins; i += NT) sh.counts[i] = 0, sh.masses[i] = 0;
+        __syncthreads();
+        const bool count = f.top_k < C, masses = f.top_p < 1;
+        each([&](float x, int) {
+            const int b = bin_of(x);
+            if (count) atomicAdd(&sh.counts[b], 1u);
+            if (masses) {
+                const uint64_t v = mass(x);
+                if (v) atomicAdd(&sh.masses[b], (unsigned long long)v);
+            }
+        });
+        __syncthreads();
+        uint64_t low = 0;
+        if (count) {
+            low = cut_at<true>((double)f.top_k, 0);
+            if (masses) {
+                // what is left of the bin, and nothing behind it
+                const int bin = bin_of(rank_score(low));
+                unsigned long long left = 0;
+                each([&](float x, int c) {
+                    if (bin_of(x) == bin && rank_key(score_key(x), c) >= low) left += mass(x);
+                });
+                left = block_sum<unsigned long long, NT>(left, sh.upart);
+                for (int i = threadIdx.x; i < kBins; i += NT)
+                    if (i >= bin) sh.masses[i] = i == bin ? left : 0;
+                __syncthreads();
+            }
+        }
+        if (masses) {
+            unsigned long long mine = 0;
+            for (int i = threadIdx.x; i < kBins; i += NT) mine += sh.masses[i];
+            const double total = (double)block_sum<unsigned long long, NT>(mine, sh.upart);
+            const double goal = f.top_p * total;
+            // (nothing to reach: the first label stays alone)
+            low = goal > 0 ? cut_at<false>(goal, low) : cut_at<true>(1.0, 0);
+        }
+        return low;
+    }
+
+    // Step 4.  cut: lowest rank key that stays
+    __device__ void draw(uint64_t cut, double min_p, float u, unsigned r, const Out &out)
+    {
+        constexpr int V = kVec<T>, step = 64 * V;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int tiles = (C + step - 1) / step, per = (tiles + kRuns - 1) / kRuns, runs = (tiles + per - 1) / per;
+        const float cut_score = cut ? rank_score(cut) : -INFINITY;
+        // a tile's kept weights
+        auto tile = [&](int t, double (&w)[V]) {
+            const int c = t * step + lane * V;
+            float x[V];
+            if (sc == 1 && c + V <= C) {
+                load_vec(p + c, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = c + i < C ? to_float(p[(c + i) * sc]) : -INFINITY;
+            }
+            float best = x[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) best = fmaxf(best, x[i]);
+            const bool some = __any(best >= cut_score && best > -INFINITY);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                w[i] = 0;
+                if (some && x[i] >= cut_score && rank_key(score_key(x[i]), c + i) >= cut) {
+                    const double v = weight(x[i]);
+                    w[i] = v >= min_p ? v : 0.0;
+                }
+            }
+            return some;
+        };
+        for (int e = wave; e < runs; e += NT / 64) {
+            double sum = 0;
+            for (int t = e * per; t < min(tiles, (e + 1) * per); ++t) {
+                double w[V];
+                if (!tile(t, w)) continue;
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum += w[i];
+            }
+            if (__any(sum > 0)) {
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+            }
+            if (lane == 0) sh.runs[e] = sum;
+        }
+        __syncthreads();
+        // the run that the draw falls into, or the last one that holds something
+        constexpr int mine = kRuns / NT > 0 ? kRuns / NT : 1;
+        double sum = 0, all;
+        int last = -1;
+        for (int i = 0; i < mine; ++i) {
+            const int e = threadIdx.x * mine + i;
+            if (e < runs && sh.runs[e] > 0) sum += sh.runs[e], last = e;
+        }
+        double front = block_front<double, NT>(sum, sh.dpart, all);
+        if (threadIdx.x == 0) sh.bin = 0, sh.listed = ~0u;
+        __syncthreads();
+        if (last >= 0) atomicMax(&sh.bin, (unsigned)last);
+        const double target = draw_of(u) * all;
+        if (sum > 0 && front + sum > target) {       // (the lowest run wins)
+            for (int i = 0; i < mine; ++i) {
+                const int e = threadIdx.x * mine + i;
+                const double next = front + (e < runs ? sh.runs[e] : 0.0);
+                if (next > target) {
+                    atomicMin(&sh.listed, (unsigned)e);
+                    break;
+                }
+                front = next;
+            }
+        }
+        __syncthreads();
+        const int run = sh.listed != ~0u ? (int)sh.listed : (int)sh.bin;
+        if (wave) return;
+        front = 0;
+        for (int i = lane; i < run; i += 64) front += sh.runs[i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) front += __shfl_xor(front, o);
+        int label = -1;
+        double got = 0;
+        for (int t = run * per; t < min(tiles, (run + 1) * per); ++t) {
+            double w[V];
+            if (!tile(t, w)) continue;
+            double own = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) own += w[i];
+            double upto = own;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double other = __shfl_up(upto, o);
+                if (lane >= o) upto += other;
+            }
+            // the first lane past the target, else the last one that holds something (so far)
+            const uint64_t past = __ballot(own > 0 && front + upto > target), holds = __ballot(own > 0);
+            if (past || holds) {
+                const int who = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)holds);
+                double run_sum = front + upto - own;
+                int l = -1;
+                double g = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const bool open = w[i] > 0 && !(l >= 0 && run_sum > target);
+                    run_sum += open ? w[i] : 0.0;
+                    l = open ? t * step + lane * V + i : l;
+                    g = open ? w[i] : g;
+                }
+                label = __shfl(l, who);
+                got = __shfl(g, who);
+            }
+            if (past) break;
+            front += __shfl(upto, 63);
+        }
+        if (lane == 0) put(out, r, label, log(got / all));
+    }
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
+sample_blocks_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+{
+    __shared__ typename BlockRow<T, NT>::Shared sh;
+    const unsigned r = blockIdx.x;
+    const RowOf<T> at(in, r);
+    const Filter f = filter_of(set, at.n, in.C);
+    const int wide = 32 - __builtin_clz(in.C);      // C < 2^wide
+    BlockRow<T, NT> row = {sh, at.p, in.sc, in.C, 0.f, 0.f, {}, min(51, 62 - wide)};
+    row.largest();
+    if (!(fabsf(row.m) < INFINITY)) {
         if (threadIdx.x == 0) put(out, r, -1, -INFINITY);
         return;
     }
-    auto weight = [&](float x) { return exp(((double)x - (double)m) * f.inv_t); };
-    uint64_t cut = 0;
-    if (f.ranked) {
-        auto search = [&](auto reached) {
-            uint64_t k = 0;
-            for (int b = 63; b >= 0; --b)
-                if (reached(k | 1ull << b)) k |= 1ull << b;
-            return k;
-        };
-        if (f.top_k < in.C)
-            cut = search([&](uint64_t k) {
-                int count = 0;
-                for (int c = threadIdx.x; c < in.C; c += kRowThreads) count += rank_key(score_key(to_float(p[c * in.sc])), c) >= k;
-                return block_sum(count, ipart) >= f.top_k;
-            });
-        if (f.top_p < 1) {
-            auto mass = [&](uint64_t k) {
-                double sum = 0;
-                for (int c = threadIdx.x; c < in.C; c += kRowThreads) {
-                    const float x = to_float(p[c * in.sc]);
-                    const uint64_t key = rank_key(score_key(x), c);
-                    if (key >= cut && key >= k) sum += weight(x);
-                }
-                return block_sum(sum, part);
-            };
-            const double goal = f.top_p * mass(0);
-            const uint64_t nucleus = search([&](uint64_t k) {
-                const double sum = mass(k);
-                return sum > 0 && sum >= goal;
-            });
-            cut = nucleus > cut ? nucleus : cut;
-        }
-    }
-    auto kept_weight = [&](float x, int c) {
-        const double w = weight(x);
-        const bool keep = (w >= f.min_p || score_key(x) == mk) && rank_key(score_key(x), c) >= cut;
-        return keep ? w : 0.0;
-    };
-    // every thread a run of neighbouring labels
-    const int chunk = (in.C + kRowThreads - 1) / kRowThreads;
-    const int c0 = threadIdx.x * chunk, c1 = min(in.C, c0 + chunk);
-    double mine = 0;
-    for (int c = c0; c < c1; ++c) mine += kept_weight(to_float(p[c * in.sc]), c);
-    sums[threadIdx.x] = mine;
+    row.scale = (float)fmin(f.inv_t * kBinsPerUnit, 1e30);
+    row.weight = {row.m, f.inv_t * kLog2eD};
+    const uint64_t cut = f.top_k < in.C || f.top_p < 1 ? row.cut(f) : 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double total = 0;
-        int last = 0;
-        for (int i = 0; i < kRowThreads; ++i) {
-            total += sums[i];
-            if (sums[i] > 0) last = i;
-        }
-        const double target = draw_of(uniform[r]) * total;
-        double run = 0, got = 0;
-        int label = -1;
-        for (int i = 0; i < kRowThreads; ++i) {
-            const double next = run + sums[i];
-            if (next > target || i == last) {
-                // (rounding may leave the target just past a run's last label: the search then goes on in the next run)
-                for (int c = i * chunk; c < in.C; ++c) {
-                    const double w = kept_weight(to_float(p[c * in.sc]), c);
-                    if (w == 0) continue;
-                    run += w;
-                    label = c;
-                    got = w;
-                    if (run > target) break;
-                }
-                break;
-            }
-            run = next;
-        }
-        put(out, r, label, log(got / total));
-    }
+    row.draw(cut, f.min_p, uniform[r], r, out);
 }
 
-template <typename T>
-int run(const Rows &in, const Settings &set, const float *uniform, const Out &out, hipStream_t st)
+// top_k for all rows, and short enough for a list (temperature 0: the best one)
+int list_length(const Settings &set)
 {
-    if (in.sc == 1 && in.C >= 512)
-        hipLaunchKernelGGL(sample_rows_kernel<T>, dim3(in.rows), dim3(kRowThreads), 0, st, in, set, uniform, out);
-    else
+    if (set.top_k_n) return 0;
+    if (!set.t_n && set.t == 0) return 1;
+    return set.top_k >= 1 && set.top_k <= MFL_MAX_TOP_LABELS ? set.top_k : 0;
+}
+bool by_lanes(const Rows &in) { return !(in.sc == 1 && in.C >= 256); }
+
+template <typename T>
+int run(const Rows &in, const Settings &set, const float *uniform, const Out &out, void *workspace, hipStream_t st)
+{
+    if (by_lanes(in)) {
         hipLaunchKernelGGL(sample_lanes_kernel<T>, dim3((in.rows + kLaneThreads - 1) / kLaneThreads), dim3(kLaneThreads), 0, st, in, set,
                            uniform, out);
+        return (int)hipGetLastError();
+    }
+    const int k = list_length(set) < in.C ? list_length(set) : 0;
+    if (k) {
+        if (in.C < kBlockLabels) {
+            const unsigned per = kWaveTopThreads / 64;
+            hipLaunchKernelGGL(list_waves_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kWaveTopThreads), 0, st, in, set, k, uniform, out);
+            return (int)hipGetLastError();
+        }
+        const int parts = top_parts(in.rows, in.C);
+        uint64_t *keys = (uint64_t *)workspace;
+        hipLaunchKernelGGL(list_parts_kernel<T>, dim3(in.rows * parts), dim3(kWaveTopThreads), 0, st, in, set, k, parts, uniform, keys, out);
+        if (parts > 1) hipLaunchKernelGGL(list_join_kernel<T>, dim3(in.rows), dim3(64), 0, st, in, set, k, parts, uniform, keys, out);
+        return (int)hipGetLastError();
+    }
+    if (in.C <= 4096) hipLaunchKernelGGL((sample_blocks_kernel<T, 256>), dim3(in.rows), dim3(256), 0, st, in, set, uniform, out);
+    else hipLaunchKernelGGL((sample_blocks_kernel<T, 1024>), dim3(in.rows), dim3(1024), 0, st, in, set, uniform, out);
     return (int)hipGetLastError();
 }
 
@@ -261,8 +680,10 @@ extern "C" {
 
 size_t mfl_sample_labels_workspace_bytes(int N, int C, int S, int dtype)
 {
-    (void)N, (void)C, (void)S, (void)dtype;
-    return 0;
+    Rows in;
+    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || C < kBlockLabels) return 0;
+    const int parts = top_parts(in.rows, in.C);
+    return parts > 1 ? (size_t)in.rows * parts * MFL_MAX_TOP_LABELS * sizeof(uint64_t) : 0;
 }
 
 int mfl_sample_labels(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c, long long stride_s,
@@ -279,15 +700,15 @@ int mfl_sample_labels(const void *scores, int dtype, int N, int C, int S, long l
     if ((!temperature_n && temperature != 0 && !temperature_ok(temperature)) || (!top_k_n && top_k < 0) ||
         (!top_p_n && !(top_p > 0 && top_p <= 1)) || (!min_p_n && !(min_p >= 0 && min_p <= 1)))
         return MFL_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < mfl_sample_labels_workspace_bytes(N, C, S, dtype)) return MFL_ERR_WORKSPACE;
-    (void)workspace;
+    const size_t need = by_lanes(in) ? 0 : mfl_sample_labels_workspace_bytes(N, C, S, dtype);
+    if (need && (!workspace || workspace_bytes < need)) return MFL_ERR_WORKSPACE;
     const Settings set = {temperature, top_p, min_p, top_k, temperature_n, top_p_n, min_p_n, top_k_n};
     const Out out = {labels, label_bytes, logprob};
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case MFL_F32: return run<float>(in, set, uniform, out, st);
-    case MFL_BF16: return run<bf16_t>(in, set, uniform, out, st);
-    default: return run<f16_t>(in, set, uniform, out, st);
+    case MFL_F32: return run<float>(in, set, uniform, out, workspace, st);
+    case MFL_BF16: return run<bf16_t>(in, set, uniform, out, workspace, st);
+    default: return run<f16_t>(in, set, uniform, out, workspace, st);
     }
 }
 

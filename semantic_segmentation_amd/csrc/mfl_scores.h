@@ -231,6 +231,30 @@ constexpr double kLog2eD = 1.44269504088896340736;
 // (log2(e) / temperature and its inverse have to be ordinary fp32 numbers)
 inline bool temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }
 
+// exp((score - m) / temperature) in 64 bits, for scores up to m: 2^y = 2^n 2^f with n = rint(y), f in [-1/2, 1/2], and the
+// Taylor polynomial of 2^f to f^11 (the next term is 2^-47).  The largest score weighs exactly 1.
+struct Weight {
+    double m, a;                // a = log2(e) / temperature
+    __device__ double operator()(float x) const
+    {
+        const double y = fmax(((double)x - m) * a, -1100.0);     // (2^-1100 is 0; -inf would leave f undefined)
+        const double n = __builtin_rint(y), f = y - n;
+        double p = 4.4455382718708117e-10;                       // ln(2)^n / n!
+        p = fma(p, f, 7.0549116208011233e-09);
+        p = fma(p, f, 1.0178086009239699e-07);
+        p = fma(p, f, 1.3215486790144309e-06);
+        p = fma(p, f, 1.5252733804059840e-05);
+        p = fma(p, f, 1.5403530393381610e-04);
+        p = fma(p, f, 1.3333558146428443e-03);
+        p = fma(p, f, 9.6181291076284772e-03);
+        p = fma(p, f, 5.5504108664821580e-02);
+        p = fma(p, f, 2.4022650695910071e-01);
+        p = fma(p, f, 6.9314718055994531e-01);
+        p = fma(p, f, 1.0);
+        return __builtin_ldexp(p, (int)n);
+    }
+};
+
 // Host: the arguments every call shares.  0 or an error code; fills the view.
 inline int make_rows(Rows &r, const void *p, int dtype, int N, int C, int S, long long sn, long long sc, long long ss)
 {
