@@ -66,65 +66,227 @@ __device__ inline void put(const Out &o, unsigned r, int label, double logprob)
 // The draw u in [0, 1): anything below counts as 0
 __device__ inline double draw_of(float u) { return u > 0 ? (double)u : 0.0; }
 
-// One lane per row.
+template <typename T> struct RowOf {
+    const T *p;
+    unsigned n;
+    __device__ RowOf(const Rows &in, unsigned r)
+    {
+        n = r / in.S;
+        p = (const T *)in.p + (long long)n * in.sn + (long long)(r - n * in.S) * in.ss;
+    }
+};
+
+// ---- one lane per row
+//
+// Without top_k and top_p the labels are streamed once, in blocks: a block's weights next to its own largest score, summed;
+// at the end the block sums are put on one scale, the draw names a block, and that block is read again for the label.  With
+// top_k or top_p the lane keeps its best labels (Best), and looks for the draw among them; where top_p needs more labels than
+// the list holds, a binary search over the rank keys finds the cut.
+
 constexpr int kLaneThreads = 256;
-template <typename T>
+constexpr int kLoneBlock = 24;          // up to this many labels a lane's scores stay in registers
+constexpr int kBlocks = 8;              // block sums a lane keeps
+constexpr int kBlock = 32;              // labels in flight
+
+template <typename T, int CB> __device__ inline void load_block(float (&x)[CB], const T *p, long long sc, int c0, int C)
+{
+    T raw[CB];
+    const T *q = p + c0 * sc;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        raw[i] = *q;
+        q += c0 + i + 1 < C ? sc : 0;           // (the last one again)
+    }
+#pragma unroll
+    for (int i = 0; i < CB; ++i) x[i] = i == 0 || c0 + i < C ? to_float(raw[i]) : -INFINITY;
+}
+template <int CB> __device__ inline float largest_of(const float (&x)[CB], float m)
+{
+#pragma unroll
+    for (int i = 0; i < CB; ++i) m = max_or_nan(m, x[i]);
+    return m;
+}
+// Weights that min_p keeps.  (No score above -inf: all 0.)
+template <int CB> __device__ inline void weights_of(double (&w)[CB], const float (&x)[CB], const Weight &weight, double min_p)
+{
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const double v = weight(x[i]);
+        w[i] = v >= min_p ? v : 0.0;
+    }
+}
+// The first of a block's labels whose running sum, from `run` on, exceeds the target, else the last that weighs something
+template <int CB> __device__ inline void pick(const double (&w)[CB], double run, double target, int &label, double &got)
+{
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const bool open = w[i] > 0 && !(label >= 0 && run > target);
+        run += open ? w[i] : 0.0;
+        label = open ? i : label;
+        got = open ? w[i] : got;
+    }
+}
+
+// All labels in registers
+template <typename T, int CB>
 __global__ void __launch_bounds__(kLaneThreads)
-sample_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+plain_lone_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
 {
     const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
     if (r >= in.rows) return;
-    const unsigned n = r / in.S, s = r - n * in.S;
-    const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
-    const Filter f = filter_of(set, n, in.C);
+    const RowOf<T> row(in, r);
+    float x[CB];
+    load_block(x, row.p, in.sc, 0, in.C);
+    const float u = uniform[r];
+    const Filter f = filter_of(set, row.n, in.C);
+    const float m = largest_of(x, -INFINITY);
+    if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
+    const Weight weight = {m, f.inv_t * kLog2eD};
+    double w[CB], total = 0;
+    weights_of(w, x, weight, f.min_p);
+#pragma unroll
+    for (int i = 0; i < CB; ++i) total += w[i];
+    int label = -1;
+    double got = 0;
+    pick(w, 0.0, draw_of(u) * total, label, got);
+    put(out, r, label, log(got / total));
+}
+
+struct LaneSums {
+    double sum[kBlocks][kLaneThreads];
+    float top[kBlocks][kLaneThreads];
+};
+template <typename T>
+__device__ inline void plain_lane(const Rows &in, const T *p, const Filter &f, float u, unsigned r, const Out &out, LaneSums &sh)
+{
+    const int per = (in.C + kBlocks * kBlock - 1) / (kBlocks * kBlock) * kBlock, blocks = (in.C + per - 1) / per;
+    const double a = f.inv_t * kLog2eD;
+    float m = -INFINITY, x[kBlock];
+    if (f.min_p > 0) {          // the threshold needs the largest score first
+        for (int c = 0; c < in.C; c += kBlock) {
+            load_block(x, p, in.sc, c, in.C);
+            m = largest_of(x, m);
+        }
+        if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
+    }
+    double w[kBlock];
+    for (int b = 0; b < blocks; ++b) {
+        double sum = 0;
+        float top = m;
+        for (int c = b * per; c < min(in.C, (b + 1) * per); c += kBlock) {
+            load_block(x, p, in.sc, c, in.C);
+            if (!(f.min_p > 0)) {
+                const float next = largest_of(x, top);
+                if (c > b * per && next != top) sum *= Weight{next, a}(top);
+                top = next;
+            }
+            // (labels of the next block, where the block's size is not a multiple of what is in flight: there are none)
+            weights_of(w, x, Weight{top == -INFINITY ? 0.0 : (double)top, a}, f.min_p);
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) sum += w[i];
+        }
+        sh.sum[b][threadIdx.x] = sum;
+        sh.top[b][threadIdx.x] = top;
+    }
+    if (!(f.min_p > 0)) {
+        for (int b = 0; b < blocks; ++b) m = max_or_nan(m, sh.top[b][threadIdx.x]);
+        if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
+    }
+    const Weight weight = {m, a};
+    double total = 0;
+    for (int b = 0; b < blocks; ++b) {
+        const double s = sh.sum[b][threadIdx.x] * weight(sh.top[b][threadIdx.x]);
+        sh.sum[b][threadIdx.x] = s;
+        total += s;
+    }
+    const double target = draw_of(u) * total;
+    double front = 0, run = 0;
+    int block = 0;
+    bool past = false;
+    for (int b = 0; b < blocks; ++b) {
+        const double s = sh.sum[b][threadIdx.x];
+        if (s > 0 && !past) {
+            block = b;
+            front = run;
+        }
+        run += s;
+        past = past || (s > 0 && run > target);
+    }
+    int label = -1;
+    double got = 0;
+    for (int c = block * per; c < min(in.C, (block + 1) * per); c += kBlock) {
+        load_block(x, p, in.sc, c, in.C);
+        weights_of(w, x, weight, f.min_p);
+        int here = -1;
+        double v = 0;
+        pick(w, front, target, here, v);
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) front += w[i];
+        if (here >= 0) {
+            label = c + here;
+            got = v;
+        }
+        if (here >= 0 && front > target) break;
+    }
+    put(out, r, label, log(got / total));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLaneThreads)
+plain_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+{
+    __shared__ LaneSums sh;
+    const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
+    if (r >= in.rows) return;
+    const RowOf<T> row(in, r);
+    plain_lane(in, row.p, filter_of(set, row.n, in.C), uniform[r], r, out, sh);
+}
+
+// The cut by a binary search over the rank keys, then the draw: for any settings
+template <typename T>
+__device__ inline void search_lane(const Rows &in, const T *p, const Filter &f, float u, unsigned r, const Out &out)
+{
     int mk = (int)0x80000000;
     for (int c = 0; c < in.C; ++c) mk = max(mk, score_key(to_float(p[c * in.sc])));
     const float m = key_score(mk);
     if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
     const Weight weight = {m, f.inv_t * kLog2eD};
+    auto search = [&](auto reached) {
+        uint64_t k = 0;
+        for (int b = 63; b >= 0; --b)
+            if (reached(k | 1ull << b)) k |= 1ull << b;
+        return k;
+    };
     uint64_t cut = 0;                               // kept by rank: rank_key >= cut
-    if (f.top_k < in.C || f.top_p < 1) {
-        // binary search over the rank keys, from the top bit down
-        auto search = [&](auto reached) {
-            uint64_t k = 0;
-            for (int b = 63; b >= 0; --b)
-                if (reached(k | 1ull << b)) k |= 1ull << b;
-            return k;
-        };
-        double total = 0;
-        if (f.top_k < in.C)
-            cut = search([&](uint64_t k) {
-                int count = 0;
-                for (int c = 0; c < in.C; ++c) count += rank_key(score_key(to_float(p[c * in.sc])), c) >= k;
-                return count >= f.top_k;
-            });
-        if (f.top_p < 1) {
+    if (f.top_k < in.C)
+        cut = search([&](uint64_t k) {
+            int count = 0;
+            for (int c = 0; c < in.C; ++c) count += rank_key(score_key(to_float(p[c * in.sc])), c) >= k;
+            return count >= f.top_k;
+        });
+    if (f.top_p < 1) {
+        auto mass = [&](uint64_t from) {
+            double sum = 0;
             for (int c = 0; c < in.C; ++c) {
                 const float x = to_float(p[c * in.sc]);
-                if (rank_key(score_key(x), c) >= cut) total += weight(x);
+                if (rank_key(score_key(x), c) >= from) sum += weight(x);
             }
-            const uint64_t top = rank_key(mk, 0);
-            const uint64_t nucleus = search([&](uint64_t k) {
-                if (k > top) return false;
-                double sum = 0;
-                for (int c = 0; c < in.C; ++c) {
-                    const float x = to_float(p[c * in.sc]);
-                    const uint64_t key = rank_key(score_key(x), c);
-                    if (key >= cut && key >= k) sum += weight(x);
-                }
-                return sum > 0 && sum >= f.top_p * total;
-            });
-            cut = nucleus > cut ? nucleus : cut;
-        }
+            return sum;
+        };
+        const double goal = f.top_p * mass(cut);
+        const uint64_t nucleus = search([&](uint64_t k) {
+            const double sum = mass(k > cut ? k : cut);
+            return sum > 0 && sum >= goal;
+        });
+        cut = nucleus > cut ? nucleus : cut;
     }
     auto kept_weight = [&](float x, int c) {
         const double w = weight(x);
-        const bool keep = (w >= f.min_p || score_key(x) == mk) && rank_key(score_key(x), c) >= cut;
-        return keep ? w : 0.0;
+        return w >= f.min_p && rank_key(score_key(x), c) >= cut ? w : 0.0;
     };
     double total = 0;
     for (int c = 0; c < in.C; ++c) total += kept_weight(to_float(p[c * in.sc]), c);
-    const double target = draw_of(uniform[r]) * total;
+    const double target = draw_of(u) * total;
     double run = 0, got = 0;
     int label = -1;
     for (int c = 0; c < in.C; ++c) {
@@ -138,6 +300,106 @@ sample_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Ou
     put(out, r, label, log(got / total));
 }
 
+// The K best of the row; MASS: also what all labels weigh, for a top_p of more than the list.  Returns false where the list
+// does not reach.
+template <typename T, int K, bool MASS>
+__device__ inline bool list_lane(const Rows &in, const T *p, const Filter &f, float u, unsigned r, const Out &out)
+{
+    Best<K> best;
+    constexpr int U = 8;
+    const double a = f.inv_t * kLog2eD;
+    double mass = 0;
+    float m = -INFINITY;
+    for (int c = 0; c < in.C; c += U) {
+        float x[U];
+        load_block(x, p, in.sc, c, in.C);
+        if (MASS) {
+            const float next = largest_of(x, m);
+            if (next != m) mass = m == -INFINITY ? 0.0 : mass * Weight{next, a}(m);
+            m = next;
+            if (m > -INFINITY) {
+                const Weight weight = {m, a};
+#pragma unroll
+                for (int i = 0; i < U; ++i) mass += weight(x[i]);
+            }
+        }
+        // (behind the last label: the lowest place of all, below every label's)
+#pragma unroll
+        for (int i = 0; i < U; ++i) best.insert(c + i < in.C ? place_of(x[i], c + i) : 0.0);
+    }
+    m = place_score(best.v[0]);
+    if (!(fabsf(m) < INFINITY)) {
+        put(out, r, -1, -INFINITY);
+        return true;
+    }
+    const Weight weight = {m, a};
+    double w[K], total = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        w[j] = j < f.top_k && best.v[j] != 0.0 ? weight(place_score(best.v[j])) : 0.0;
+        total += w[j];
+    }
+    if (MASS && f.top_k > K) total = mass;
+    const double goal = f.top_p * total;
+    double front = 0, sum = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const bool keep = j == 0 || ((f.top_p >= 1 || front < goal) && w[j] >= f.min_p);
+        front += w[j];
+        w[j] = keep ? w[j] : 0.0;
+        sum += w[j];
+    }
+    if (MASS && f.top_k > K && in.C > K && (f.top_p >= 1 || front < goal)) return false;
+    // label by label, in label order, until the running sum is past the target
+    const double target = draw_of(u) * sum;
+    double run = 0, got = 0;
+    int label = -1;
+    for (;;) {
+        int next = 0x7fffffff;
+        double v = 0;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int l = place_label(best.v[j]);
+            const bool here = w[j] > 0 && l > label && l < next;
+            next = here ? l : next;
+            v = here ? w[j] : v;
+        }
+        if (next == 0x7fffffff) break;
+        run += v;
+        label = next;
+        got = v;
+        if (run > target) break;
+    }
+    put(out, r, label, log(got / sum));
+    return true;
+}
+
+template <typename T, int K>
+__global__ void __launch_bounds__(kLaneThreads)
+list_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+{
+    const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
+    if (r >= in.rows) return;
+    const RowOf<T> row(in, r);
+    list_lane<T, K, false>(in, row.p, filter_of(set, row.n, in.C), uniform[r], r, out);
+}
+
+// Any settings, of each n its own
+constexpr int kAnyList = 16;
+template <typename T>
+__global__ void __launch_bounds__(kLaneThreads)
+any_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+{
+    __shared__ LaneSums sh;
+    const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
+    if (r >= in.rows) return;
+    const RowOf<T> row(in, r);
+    const Filter f = filter_of(set, row.n, in.C);
+    const float u = uniform[r];
+    if (f.top_k >= in.C && f.top_p >= 1) return plain_lane(in, row.p, f, u, r, out, sh);
+    if (in.C <= kBestLabels && (f.top_k <= kAnyList || f.top_k >= in.C) && list_lane<T, kAnyList, true>(in, row.p, f, u, r, out)) return;
+    search_lane(in, row.p, f, u, r, out);
+}
 
 // ---- rows that top_k cuts to a short list
 
@@ -220,16 +482,6 @@ __device__ inline void draw_from_list(const WaveTop<REST> &top, const Filter &f,
     for (int h = 0; h < 2; ++h)
         if (key[h] && rank_label(key[h]) == label) put(out, r, label, log(w[h] / total));
 }
-
-template <typename T> struct RowOf {
-    const T *p;
-    unsigned n;
-    __device__ RowOf(const Rows &in, unsigned r)
-    {
-        n = r / in.S;
-        p = (const T *)in.p + (long long)n * in.sn + (long long)(r - n * in.S) * in.ss;
-    }
-};
 
 template <typename T>
 __global__ void __launch_bounds__(kWaveTopThreads)
@@ -652,8 +904,27 @@ template <typename T>
 int run(const Rows &in, const Settings &set, const float *uniform, const Out &out, void *workspace, hipStream_t st)
 {
     if (by_lanes(in)) {
-        hipLaunchKernelGGL(sample_lanes_kernel<T>, dim3((in.rows + kLaneThreads - 1) / kLaneThreads), dim3(kLaneThreads), 0, st, in, set,
-                           uniform, out);
+        const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
+#define MFL_LANES(...) hipLaunchKernelGGL(__VA_ARGS__, grid, block, 0, st, in, set, uniform, out)
+        // what the list has to hold: top_k, or with top_p alone every label
+        const bool no_k = !set.top_k_n && (set.top_k == 0 || set.top_k >= in.C), no_p = !set.top_p_n && set.top_p == 1;
+        const bool same_t = !set.t_n && set.t > 0, below_1 = !set.min_p_n;
+        const int k = list_length(set) ? list_length(set) : no_k && in.C <= 32 ? in.C : 0;
+        if (no_k && no_p && same_t && below_1) {
+            if (in.C <= 8) MFL_LANES((plain_lone_kernel<T, 8>));
+            else if (in.C <= kLoneBlock) MFL_LANES((plain_lone_kernel<T, kLoneBlock>));
+            else MFL_LANES((plain_lanes_kernel<T>));
+        } else if (k && k <= 32 && in.C <= kBestLabels) {
+            if (k <= 1) MFL_LANES((list_lanes_kernel<T, 1>));
+            else if (k <= 4) MFL_LANES((list_lanes_kernel<T, 4>));
+            else if (k <= 8) MFL_LANES((list_lanes_kernel<T, 8>));
+            else if (k <= 16) MFL_LANES((list_lanes_kernel<T, 16>));
+            else if (k <= 24) MFL_LANES((list_lanes_kernel<T, 24>));
+            else MFL_LANES((list_lanes_kernel<T, 32>));
+        } else {
+            MFL_LANES((any_lanes_kernel<T>));
+        }
+#undef MFL_LANES
         return (int)hipGetLastError();
     }
     const int k = list_length(set) < in.C ? list_length(set) : 0;
