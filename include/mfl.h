@@ -368,7 +368,7 @@ int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long
  * twice counts as two entries.  Rows with valid = 0, without any teacher mass or whose scores are all -inf have loss 0
  * and gradient 0, whatever the other tensors hold there.
  *   values: [N][k][S] of values_dtype   labels: [N][k][S] int32   rest: [N][S] float or NULL (entries renormalised)
- *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [4][N][S] floats, from forward to backward
+ *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [5][N][S] floats, from forward to backward
  *   grad_loss: [N][S]   d_scores: the scores' type, with strides of its own, overwritten
  */
 size_t mfl_distillation_workspace_bytes(int N, int C, int S, int dtype, int k);

@@ -37,6 +37,7 @@ constexpr int kLaneThreads = 256;
 // The teacher's distribution of a row.  log p_j = (t_j - m) / T - l, log p_rest = rest - m / T - l
 struct Target {
     float m, l, log_p_rest, p_rest;
+    float s;                    // l = log(1 + s)
     bool any;                   // it holds something
 };
 // sum: the entries with a label of the row (named: there are some); rest: -inf for none
@@ -45,12 +46,12 @@ __device__ inline Target target_of(const Teacher &t, Excess sum, bool named, flo
     Target g;
     if (sum.m == -INFINITY && rest != -INFINITY) sum.m = rest * t.t;
     const float above = fmaf(-sum.m, t.inv_t, rest);       // the rest next to the largest entry
-    if (rest == -INFINITY) g.l = log_1p(sum.s);
-    else if (above <= 0) g.l = log_1p(sum.s + __builtin_amdgcn_exp2f(above * kLog2e));
-    else g.l = above + log_1p((1.f + sum.s) * __builtin_amdgcn_exp2f(-above * kLog2e));
+    g.s = rest == -INFINITY ? sum.s : sum.s + __builtin_amdgcn_exp2f(above * kLog2e);
+    g.l = rest == -INFINITY || above <= 0 ? log_1p(g.s) : above + log_1p((1.f + sum.s) * __builtin_amdgcn_exp2f(-above * kLog2e));
     g.m = sum.m;
     g.any = named && !(sum.m == -INFINITY && sum.s == -1.f);
-    g.log_p_rest = rest == -INFINITY ? -INFINITY : above - g.l;
+    const float ratio = (1.f + sum.s) * __builtin_amdgcn_exp2f(-above * kLog2e);        // the record next to the rest
+    g.log_p_rest = rest == -INFINITY ? -INFINITY : ratio == INFINITY ? above - g.l : -log_1p(ratio);
     g.p_rest = __builtin_amdgcn_exp2f(g.log_p_rest * kLog2e);
     return g;
 }
@@ -58,22 +59,37 @@ __device__ inline float log_share(const Teacher &t, const Target &g, float value
 
 // p (log p - log q); nothing where p is 0
 __device__ inline float share_term(float p, float log_p, float log_q) { return p == 0.f ? 0.f : p * (log_p - log_q); }
+// ... of an entry: log p - log q = ((t - m_p) - (score - m_q)) / T - log((1 + s_p) / (1 + s_q)), in this order, since close
+// to the teacher the two logarithms agree in most of their digits
+__device__ inline float entry_term(const Teacher &t, const Target &g, float log_sums, float m, float value, float x)
+{
+    const float p = __builtin_amdgcn_exp2f(log_share(t, g, value) * kLog2e);
+    return p == 0.f ? 0.f : p * fmaf((value - g.m) - (x - m), t.inv_t, -log_sums);
+}
 
 struct Stats {
-    float m, z, mo, zo;         // as above
+    float m, z, mo, zo, log_q_rest;     // as above
+    float s;                            // z = log(1 + s); not kept
 };
-constexpr Stats kNoStats = {-INFINITY, 0.f, -INFINITY, 0.f};
-// top: the record's labels, each once; out: all others
-__device__ inline Stats stats_of(Excess top, LogSum out, float c2)
+constexpr Stats kNoStats = {-INFINITY, 0.f, -INFINITY, 0.f, -INFINITY, 0.f};
+// log((1 + s_p) / (1 + s_q))
+__device__ inline float log_sums(const Target &g, const Stats &a)
 {
-    const Excess all = join(top, Excess{out.m, out.s - 1.f}, c2);
-    if (all.m == -INFINITY && all.s == -1.f) return kNoStats;
-    const bool some = !(out.m == -INFINITY && out.s == 0.f);
-    return {all.m, log_1p(all.s), some ? out.m : -INFINITY, some ? logf(out.s) : 0.f};
+    const float d = (g.s - a.s) / (1.f + a.s);
+    return fabsf(d) < 0.5f ? log_1p(d) : g.l - a.z;
 }
-__device__ inline float log_q_rest(const Stats &a, float inv_t)
+// top: the record's labels, each once; out: all others
+__device__ inline Stats stats_of(Excess top, LogSum out, const Teacher &t)
 {
-    return a.mo == -INFINITY ? -INFINITY : (a.mo - a.m) * inv_t + (a.zo - a.z);
+    const Excess all = join(top, Excess{out.m, out.s - 1.f}, t.c2);
+    if (all.m == -INFINITY && all.s == -1.f) return kNoStats;
+    Stats a = {all.m, log_1p(all.s), -INFINITY, 0.f, -INFINITY, all.s};
+    if (out.m == -INFINITY && out.s == 0.f) return a;
+    a.mo = out.m;
+    a.zo = logf(out.s);
+    const float ratio = (1.f + top.s) * __builtin_amdgcn_exp2f((top.m - out.m) * t.c2) / out.s;
+    a.log_q_rest = ratio == INFINITY ? (a.mo - a.m) * t.inv_t + (a.zo - a.z) : -log_1p(ratio);
+    return a;
 }
 __device__ inline void put(float *loss, float *stats, size_t rows, unsigned r, float l, const Stats &a)
 {
@@ -83,10 +99,11 @@ __device__ inline void put(float *loss, float *stats, size_t rows, unsigned r, f
     stats[rows + r] = a.z;
     stats[2 * rows + r] = a.mo;
     stats[3 * rows + r] = a.zo;
+    stats[4 * rows + r] = a.log_q_rest;
 }
 __device__ inline Stats load_stats(const float *stats, size_t rows, unsigned r)
 {
-    return {stats[r], stats[rows + r], stats[2 * rows + r], stats[3 * rows + r]};
+    return {stats[r], stats[rows + r], stats[2 * rows + r], stats[3 * rows + r], stats[4 * rows + r], 0.f};
 }
 
 // What a label's gradient is made of:  up * (exp(..top) - taken)  in the record,  f_out * exp(..out)  outside
@@ -102,7 +119,10 @@ __device__ inline Slope slope_of(const Stats &a, const Teacher &t, const Target 
     if (t.rest) {
         s.f_out = 0.f;
         if (a.mo != -INFINITY) {
-            s.f_out = s.up * (__builtin_amdgcn_exp2f(log_q_rest(a, t.inv_t) * kLog2e) - g.p_rest);
+            // q_rest - p_rest = p_rest (exp(d) - 1), exp(d) - 1 from the rounded exponential and its own logarithm (Kahan)
+            const float d = a.log_q_rest - g.log_p_rest, e = __builtin_amdgcn_exp2f(d * kLog2e);
+            const float grow = e == 1.f ? d : (e - 1.f) * (d / logf(e));
+            s.f_out = s.up * (fabsf(d) < 0.5f ? g.p_rest * grow : __builtin_amdgcn_exp2f(a.log_q_rest * kLog2e) - g.p_rest);
             s.m_out = a.mo;
             s.o_out = -a.zo * kLog2e;
         }
@@ -261,14 +281,14 @@ forward_lanes_kernel(Rows in, Teacher t, float *__restrict__ loss, float *__rest
         load_labels(x, in, p, c0);
     }
     const Target g = record.target(flags.rest(t));
-    const Stats a = stats_of(top, out, t.c2);
+    const Stats a = stats_of(top, out, t);
     if (!flags.valid(t) || !g.any || a.m == -INFINITY) return put(loss, LONE ? nullptr : stats, in.rows, r, 0.f, kNoStats);
-    float sum = t.rest ? share_term(g.p_rest, g.log_p_rest, log_q_rest(a, t.inv_t)) : 0.f;
+    const float dl = log_sums(g, a);
+    float sum = t.rest ? share_term(g.p_rest, g.log_p_rest, a.log_q_rest) : 0.f;
     record.each([&](const Block<T, KB> &b) {
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
-            const float lp = log_share(t, g, b.value[j]), lq = (b.x[j] - a.m) * t.inv_t - a.z;
-            sum += b.label[j] >= 0 ? share_term(__builtin_amdgcn_exp2f(lp * kLog2e), lp, lq) : 0.f;
+            sum += b.label[j] >= 0 ? entry_term(t, g, dl, a.m, b.value[j], b.x[j]) : 0.f;
         }
     });
     put(loss, LONE ? nullptr : stats, in.rows, r, t.t * t.t * sum, a);
@@ -297,7 +317,7 @@ backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const
         LogSum other = {-INFINITY, 0.f};
         Excess top = kNoExcess;
         add_labels(record, x, 0, t.c2, other, top);
-        a = stats_of(top, other, t.c2);
+        a = stats_of(top, other, t);
     } else {
         a = load_stats(stats, in.rows, r);
     }
@@ -493,21 +513,18 @@ finish_rows_kernel(Rows in, Teacher t, int parts, const LogSum *__restrict__ sum
     for (int h = 0; h < 2; ++h)
         if (e.in[h] && !again[h]) top = join(top, Excess{x[h], 0.f}, t.c2);
     top = wave_join(top, t.c2);
-    const Stats a = stats_of(top, out, t.c2);
+    const Stats a = stats_of(top, out, t);
     if (a.m == -INFINITY) {
         if (lane == 0) put(loss, stats, in.rows, r, 0.f, a);
         return;
     }
+    const float dl = log_sums(g, a);
     float sum = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (!e.in[h]) continue;
-        const float lp = log_share(t, g, e.value[h]), lq = (x[h] - a.m) * t.inv_t - a.z;
-        sum += share_term(__builtin_amdgcn_exp2f(lp * kLog2e), lp, lq);
-    }
+    for (int h = 0; h < 2; ++h) sum += e.in[h] ? entry_term(t, g, dl, a.m, e.value[h], x[h]) : 0.f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (t.rest) sum += share_term(g.p_rest, g.log_p_rest, log_q_rest(a, t.inv_t));
+    if (t.rest) sum += share_term(g.p_rest, g.log_p_rest, a.log_q_rest);
     if (lane == 0) put(loss, stats, in.rows, r, t.t * t.t * sum, a);
 }
 

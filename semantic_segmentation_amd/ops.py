@@ -247,7 +247,7 @@ def _record(scores, top_scores, top_labels, rest, valid):
 
 def _distillation_forward(scores, v, args, record, rows, temperature):
     loss = torch.empty(rows, dtype=torch.float32, device=scores.device)
-    stats = torch.empty((4,) + rows, dtype=torch.float32, device=scores.device)
+    stats = torch.empty((5,) + rows, dtype=torch.float32, device=scores.device)
     n = lib.mfl_distillation_workspace_bytes(*args[2:5], args[1], record[5])
     ws = torch.empty(n, dtype=torch.uint8, device=scores.device) if n else None
     _lib.call_scores(lib.mfl_distillation_forward, "mfl_distillation_forward", v, *args, *record, temperature, loss.data_ptr(),
@@ -281,7 +281,7 @@ def distillation_backward(scores, top_scores, top_labels, stats, grad_loss, rest
     the other arguments as there, stats as it returned them."""
     v, args = _score_rows(scores)
     _, record, rows = _record(scores, top_scores, top_labels, rest, valid)
-    stats = _beside(scores, stats, "stats", _F32, (4,) + rows)
+    stats = _beside(scores, stats, "stats", _F32, (5,) + rows)
     grad_loss = _beside(scores, grad_loss, "grad_loss", _F32, rows)
     return _distillation_backward(scores, v, args, record, stats, grad_loss, temperature)
 
