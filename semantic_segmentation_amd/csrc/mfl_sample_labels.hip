@@ -401,7 +401,7 @@ any_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out o
     search_lane(in, row.p, f, u, r, out);
 }
 
-// ---- rows that top_k cuts to a short list
+// ---- rows that top_k cuts to a short list: of at most k labels (rows of a longer one are passed over)
 
 // One wave: draws from the list (at most 128 keys, in any order) of the row's best labels
 template <bool REST>
@@ -432,23 +432,33 @@ __device__ inline void draw_from_list(const WaveTop<REST> &top, const Filter &f,
         share[lane + 64 * h] = w[h];
     }
     __builtin_amdgcn_wave_barrier();
-    if (f.top_p < 1 || f.min_p > 0 || f.top_k < top.count) {
-        double front[2] = {0, 0}, total = 0;
+    if (f.top_k < top.count) {
         int above[2] = {0, 0};
+        for (int j = 0; j < top.count; ++j) {
+            const uint64_t other = top.list[j];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) above[h] += other > key[h];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            w[h] = above[h] < f.top_k ? w[h] : 0.0;
+            share[lane + 64 * h] = w[h];
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    if (f.top_p < 1 || f.min_p > 0) {
+        double front[2] = {0, 0}, total = 0;
         for (int j = 0; j < top.count; ++j) {
             const uint64_t other = top.list[j];
             const double v = share[j];
             total += v;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                front[h] += other > key[h] ? v : 0.0;
-                above[h] += other > key[h];
-            }
+            for (int h = 0; h < 2; ++h) front[h] += other > key[h] ? v : 0.0;
         }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const bool keep = key[h] == best || (above[h] < f.top_k && (front[h] < f.top_p * total || f.top_p >= 1) && w[h] >= f.min_p);
+            const bool keep = key[h] == best || ((front[h] < f.top_p * total || f.top_p >= 1) && w[h] >= f.min_p);
             w[h] = keep ? w[h] : 0.0;
             share[lane + 64 * h] = w[h];
         }
@@ -493,7 +503,9 @@ list_waves_kernel(Rows in, Settings set, int k, const float *__restrict__ unifor
     const unsigned r = blockIdx.x * (kWaveTopThreads / 64) + wave;
     if (r >= in.rows) return;
     const RowOf<T> row(in, r);
-    WaveTop<false> top(lists[wave], k, 0.f);
+    const Filter f = filter_of(set, row.n, in.C);
+    if (f.top_k > k) return;
+    WaveTop<false> top(lists[wave], f.top_k, 0.f);
     if (in.sc == 1 && in.C >= 8 * 64 * kVec<T>) {
         float m[4];
         top.look(row.p, 0, 4, m);
@@ -501,7 +513,7 @@ list_waves_kernel(Rows in, Settings set, int k, const float *__restrict__ unifor
     }
     top.stream(row.p, in.sc, 0, in.C);
     top.cut();
-    draw_from_list(top, filter_of(set, row.n, in.C), uniform[r], r, out, (lds_double *)share[wave]);
+    draw_from_list(top, f, uniform[r], r, out, (lds_double *)share[wave]);
 }
 
 template <typename T>
@@ -513,43 +525,54 @@ list_parts_kernel(Rows in, Settings set, int k, int parts, const float *__restri
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
     const RowOf<T> row(in, r);
-    WaveTop<false> top(sh.lists[wave], k, 0.f);
+    const Filter f = filter_of(set, row.n, in.C);
+    if (f.top_k > k) return;
+    WaveTop<false> top(sh.lists[wave], f.top_k, 0.f);
     const int size = top_part_labels(in.C, parts);
     const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
     if (!top_of_part(top, sh, row.p, in.sc, begin, end)) return;
-    if (parts == 1) return draw_from_list(top, filter_of(set, row.n, in.C), uniform[r], r, out, (lds_double *)share);
-    for (int j = lane; j < k; j += 64) keys[(size_t)blockIdx.x * k + j] = j < top.count ? top.list[j] : 0;
+    if (parts == 1) {
+        top.cut();
+        return draw_from_list(top, f, uniform[r], r, out, (lds_double *)share);
+    }
+    const int slots = part_keys(k);
+    for (int j = lane; j < slots; j += 64) keys[(size_t)blockIdx.x * slots + j] = j < top.count ? top.list[j] : 0;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(kWaveTopThreads)
 list_join_kernel(Rows in, Settings set, int k, int parts, const float *__restrict__ uniform, const uint64_t *__restrict__ keys, Out out)
 {
-    __shared__ uint64_t list[kListKeys];
+    __shared__ TopShared sh;
     __shared__ double share[MFL_MAX_TOP_LABELS];
     const unsigned r = blockIdx.x;
-    WaveTop<false> top(list, k, 0.f);
-    top.join(keys + (size_t)r * parts * k, parts * k);
+    const int n = parts * part_keys(k);
+    const Filter f = filter_of(set, r / in.S, in.C);
+    if (f.top_k > k) return;
+    WaveTop<false> top(sh.lists[threadIdx.x >> 6], f.top_k, 0.f);
+    if (!top_of_keys(top, sh, keys + (size_t)r * n, n)) return;
     top.cut();
-    draw_from_list(top, filter_of(set, r / in.S, in.C), uniform[r], r, out, (lds_double *)share);
+    draw_from_list(top, f, uniform[r], r, out, (lds_double *)share);
 }
 
 // ---- rows of many labels, any settings: one workgroup per row
 //
 //   1  the largest score
-//   2  where top_k or top_p cut: a histogram over 2048 bins of (largest - score) / T, 32 a unit: counts, and masses as
-//      64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose sums do not depend on the
+//   2  where top_k or top_p cut: a histogram over 4096 bins of (largest - score) / T, 128 a unit (a quarter of that for short
+//      rows): counts, and masses as 64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose sums do not depend on the
 //      order of the atomics; running sums over the bins name the bin that the cut falls into
 //   3  that bin's labels, a list in LDS; every one counts what lies above it in the list, and the lowest that stays is the
-//      cut.  (A bin of more labels than the list holds, all of nearly one score: a binary search over the rank keys.)
-//   4  the kept weights summed in runs of neighbouring labels, the run that the draw falls into, the label in it
+//      cut.  (A bin of more labels than the list holds, all of nearly one score: a binary search over the rank keys.)  On the
+//      way the weights above the bin are summed in runs of neighbouring labels
+//   4  the run that the draw falls into, and the label in it
 //
-// Steps 2 to 4 read the row again, from the caches if it fits.  Weights below the cut cost a compare in step 4.
+// Steps 2 and 3 read the row again, from the caches if it fits; scores below the cut cost a compare in step 3.
 
-constexpr int kBins = 2048;
-constexpr float kBinsPerUnit = 32.f;
-constexpr int kRuns = 1024;
+// (all of it in one function, so that what lies in LDS is known to)
+#define MFL_INLINE __device__ __attribute__((always_inline))
+
+constexpr int kRuns = 256;
 constexpr int kBinList = 2048;
+constexpr float kUnits = 32.f;          // what the bins cover
 
 template <typename V, int NT> __device__ inline V block_sum(V v, V *part)
 {
@@ -586,11 +609,13 @@ template <typename V, int NT> __device__ inline V block_front(V v, V *part, V &a
 }
 
 template <typename T, int NT> struct BlockRow {
+    static constexpr int kBins = 4 * NT, V = kVec<T>, step = 64 * V, waves = NT / 64;
     struct Shared {
         uint32_t counts[kBins];
         unsigned long long masses[kBins];
         unsigned long long key[kBinList], key_mass[kBinList];
         double runs[kRuns];
+        unsigned long long more[kRuns];         // fixed point
         unsigned long long upart[NT / 64];
         double dpart[NT / 64];
         float fpart[NT / 64];
@@ -604,19 +629,34 @@ template <typename T, int NT> struct BlockRow {
     float m, scale;
     Weight weight;
     int bits;                   // of the fixed-point masses
+    int tiles, per, count_runs; // 64 lanes' vectors of labels, tiles a run, runs
 
-    __device__ int bin_of(float x) const { return min((int)((m - x) * scale), kBins - 1); }
-    __device__ uint64_t mass(float x) const
+    MFL_INLINE BlockRow(Shared &sh, const T *p, long long sc, int C) : sh(sh), p(p), sc(sc), C(C)
+    {
+        const int wide = 32 - __builtin_clz(C);     // C < 2^wide
+        bits = min(51, 62 - wide);
+        tiles = (C + step - 1) / step;
+        per = (tiles + kRuns - 1) / kRuns;
+        count_runs = (tiles + per - 1) / per;
+    }
+    MFL_INLINE void set(const Filter &f)
+    {
+        scale = (float)fmin(f.inv_t * (kBins / kUnits), 1e30);
+        weight = {m, f.inv_t * kLog2eD};
+    }
+
+    MFL_INLINE int bin_of(float x) const { return min((int)((m - x) * scale), kBins - 1); }
+    MFL_INLINE uint64_t mass(float x) const
     {
         // 2^52 + an integer below 2^52: the low bits of the sum are that integer
         const double v = __builtin_ldexp(weight(x), bits) + 4503599627370496.0;
         return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
     }
     // f(score, label) over the row
-    template <typename F> __device__ void each(F f) const
+    template <typename F> MFL_INLINE void each(F f) const
     {
         if (sc == 1) {
-            constexpr int V = kVec<T>, U = 2;
+            constexpr int U = 2;
             int c = threadIdx.x * V;
             for (; c + (U - 1) * NT * V + V <= C; c += U * NT * V) {
                 float x[U][V];
@@ -642,10 +682,10 @@ template <typename T, int NT> struct BlockRow {
         }
     }
 
-    __device__ void largest()
+    MFL_INLINE void largest()
     {
         float v = -INFINITY;
-        each([&](float x, int) { v = max_or_nan(v, x); });
+        each([&](float x, int) __attribute__((always_inline)) { v = max_or_nan(v, x); });
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) v = max_or_nan(v, __shfl_xor(v, o));
         if ((threadIdx.x & 63) == 0) sh.fpart[threadIdx.x >> 6] = v;
@@ -654,88 +694,196 @@ template <typename T, int NT> struct BlockRow {
         m = v;
     }
 
-    // The lowest rank key that stays, where labels of at least `low` stay while front < goal, front = what the labels above
-    // hold: their number (COUNT) or mass.  The sum over everything is at least goal.
-    template <bool COUNT> __device__ uint64_t cut_at(double goal, uint64_t low)
+    // A lane's vector of a tile (behind the last label: -inf)
+    MFL_INLINE void load_tile(float (&x)[V], int t) const
     {
-        // the bin it falls into, and what the bins in front of it hold
-        constexpr int per = kBins / NT;
-        unsigned long long mine = 0, all;
-        for (int i = 0; i < per; ++i) mine += COUNT ? sh.counts[threadIdx.x * per + i] : sh.masses[threadIdx.x * per + i];
-        unsigned long long front = block_front<unsigned long long, NT>(mine, sh.upart, all);
-        if (threadIdx.x == 0) sh.listed = 0, sh.low_key = ~0ull;
-        if ((double)front < goal && (double)(front + mine) >= goal) {
-            int b = threadIdx.x * per;
-            for (;; ++b) {
-                const unsigned long long here = COUNT ? sh.counts[b] : sh.masses[b];
-                if ((double)(front + here) >= goal) break;
-                front += here;
+        const int c = t * step + (threadIdx.x & 63) * V;
+        if (sc == 1 && c + V <= C) {
+            load_vec(p + c, x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = c + i < C ? to_float(p[(c + i) * sc]) : -INFINITY;
+        }
+    }
+    // sh.runs = sums of f(vector, its first label) over the runs.  A wave takes four runs at a time, to have four loads in
+    // flight.  f is called by whole waves.
+    template <typename F> MFL_INLINE void sum_runs(F f)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        constexpr int U = 4;
+#pragma unroll 1
+        for (int e = wave; e < count_runs; e += U * waves) {
+            double sum[U] = {};
+#pragma unroll 1
+            for (int t = 0; t < per; ++t) {
+                float x[U][V];
+#pragma unroll
+                for (int u = 0; u < U; ++u) load_tile(x[u], min((e + u * waves) * per + t, tiles - 1));
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int at = (e + u * waves) * per + t;
+                    if (at < tiles) sum[u] += f(x[u], at * step + lane * V);
+                }
             }
-            sh.bin = b;
-            sh.bin_front = front;
-        }
-        __syncthreads();
-        const int bin = sh.bin;
-        front = sh.bin_front;
-        each([&](float x, int c) {
-            if (bin_of(x) != bin) return;
-            const uint64_t key = rank_key(score_key(x), c);
-            if (key < low) return;
-            const unsigned at = atomicAdd(&sh.listed, 1u);
-            if (at >= (unsigned)kBinList) return;
-            sh.key[at] = key;
-            sh.key_mass[at] = COUNT ? 1 : mass(x);
-        });
-        __syncthreads();
-        const int n = sh.listed;
-        if (n <= kBinList) {
-            for (int i = threadIdx.x; i < n; i += NT) {
-                const uint64_t key = sh.key[i];
-                unsigned long long above = 0;
-                for (int j = 0; j < n; ++j) above += sh.key[j] > key ? sh.key_mass[j] : 0;
-                if ((double)(front + above) < goal) atomicMin(&sh.low_key, key);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) sum[u] += __shfl_xor(sum[u], o);
             }
-            __syncthreads();
-            return sh.low_key;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (lane == 0 && e + u * waves < count_runs) sh.runs[e + u * waves] = sum[u];
         }
-        // the largest key from which on at least `goal` is held
-        uint64_t best = 0;
-        for (int b = 63; b >= 0; --b) {
-            const uint64_t at = best | 1ull << b, from = at > low ? at : low;
-            unsigned long long held = 0;
-            each([&](float x, int c) {
-                if (bin_of(x) == bin && rank_key(score_key(x), c) >= from) held += COUNT ? 1 : mass(x);
-            });
-            held = block_sum<unsigned long long, NT>(held, sh.upart);
-            if ((double)(front + held) >= goal) best = at;
-        }
-        return best > low ? best : low;
     }
 
-    // The lowest rank key that top_k and top_p keep
-    __device__ uint64_t cut(const Filter &f)
+    // The lowest score of bins 0 .. b (they grow as the score falls); b = -1: none
+    MFL_INLINE float lowest_of(int b) const
     {
-        for (int i = threadIdx.x; i < kBins; i += NT) sh.counts[i] = 0, sh.masses[i] = 0;
-        __syncthreads();
-        const bool count = f.top_k < C, masses = f.top_p < 1;
-        each([&](float x, int) {
-            const int b = bin_of(x);
-            if (count) atomicAdd(&sh.counts[b], 1u);
-            if (masses) {
-                const uint64_t v = mass(x);
-                if (v) atomicAdd(&sh.masses[b], (unsigned long long)v);
+        if (b < 0) return INFINITY;
+        int lo = score_key(-INFINITY), hi = score_key(m);       // hi is in, lo is not
+        if (bin_of(-INFINITY) <= b) return -INFINITY;
+#pragma unroll 1
+        while (hi - (long long)lo > 1) {
+            const int mid = (int)(((long long)lo + hi) >> 1);
+            if (bin_of(key_score(mid)) <= b) hi = mid;
+            else lo = mid;
+        }
+        return key_score(hi);
+    }
+
+    // sh.runs = the runs' weights of at least min_p of scores from `sure` on, and, unless LIST, of scores from `open` on
+    // whose key is at least cut; with LIST those labels between are listed
+    template <bool LIST> MFL_INLINE void sweep(float sure, float open, uint64_t cut, double min_p)
+    {
+        sum_runs([&](const float (&x)[V], int c) __attribute__((always_inline)) {
+            uint32_t todo = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) todo |= x[i] >= open ? 1u << i : 0u;
+            if (c + V > C) todo &= (1u << max(C - c, 0)) - 1;
+            double sum = 0;
+            // every lane its first, then its second: seldom more, where few are kept
+#pragma unroll 1
+            while (__any(todo != 0)) {
+                const int i = __ffs(todo) - 1;
+                float v = x[0];
+#pragma unroll
+                for (int j = 1; j < V; ++j) v = i == j ? x[j] : v;
+                bool keep = todo != 0;
+                todo &= todo - 1;
+                if (keep && !(v >= sure)) {
+                    const uint64_t key = rank_key(score_key(v), c + i);
+                    keep = key >= cut;
+                    if (LIST && keep) {
+                        keep = false;
+                        const unsigned at = atomicAdd(&sh.listed, 1u);
+                        if (at < (unsigned)kBinList) sh.key[at] = key;
+                    }
+                }
+                const double w = weight(v);
+                sum += keep && w >= min_p ? w : 0.0;
             }
+            return sum;
         });
         __syncthreads();
-        uint64_t low = 0;
-        if (count) {
-            low = cut_at<true>((double)f.top_k, 0);
-            if (masses) {
+    }
+
+    // The lowest rank key that top_k and top_p keep (0: all); sh.runs becomes the runs' kept weights
+    MFL_INLINE uint64_t cut_of(const Filter &f)
+    {
+        const bool by_count = f.top_k < C, by_mass = f.top_p < 1;
+        int bin = 0;
+        float sure = -INFINITY, open = -INFINITY;
+        uint64_t cut = 0;
+        bool summed = false;
+        if (by_count || by_mass) {
+            for (int i = threadIdx.x; i < kBins; i += NT) sh.counts[i] = 0, sh.masses[i] = 0;
+            __syncthreads();
+            each([&](float x, int) __attribute__((always_inline)) {
+                const int b = bin_of(x);
+                if (by_count) atomicAdd(&sh.counts[b], 1u);
+                if (by_mass) {
+                    const uint64_t v = mass(x);
+                    if (v) atomicAdd(&sh.masses[b], (unsigned long long)v);
+                }
+            });
+            __syncthreads();
+        }
+        // first by number, then by mass among what is left
+#pragma unroll 1
+        for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {
+            const bool count = stage == 0, final = stage == 1 || !by_mass;
+            // the bin it falls into, and what the bins in front of it hold
+            constexpr int each_bins = kBins / NT;
+            unsigned long long mine = 0, all;
+            for (int i = 0; i < each_bins; ++i) {
+                const int b = threadIdx.x * each_bins + i;
+                mine += count ? sh.counts[b] : sh.masses[b];
+            }
+            unsigned long long front = block_front<unsigned long long, NT>(mine, sh.upart, all);
+            // labels stay while what lies in front of them is below the goal
+            const double goal = count ? (double)f.top_k : f.top_p * (double)all;
+            if (threadIdx.x == 0) sh.listed = 0, sh.low_key = ~0ull, sh.bin = 0, sh.bin_front = 0;
+            __syncthreads();
+            if ((double)front < goal && (double)(front + mine) >= goal) {
+                int b = threadIdx.x * each_bins;
+                for (;; ++b) {
+                    const unsigned long long here = count ? sh.counts[b] : sh.masses[b];
+                    if ((double)(front + here) >= goal) break;
+                    front += here;
+                }
+                sh.bin = b;
+                sh.bin_front = front;
+            }
+            for (int i = threadIdx.x; i < kRuns; i += NT) sh.more[i] = 0;
+            __syncthreads();
+            bin = sh.bin;
+            front = sh.bin_front;
+            sure = lowest_of(bin - 1);
+            open = lowest_of(bin);
+            sweep<true>(sure, open, cut, f.min_p);
+            const int n = sh.listed;
+            if (n <= kBinList) {
+                for (int i = threadIdx.x; i < n; i += NT) sh.key_mass[i] = count ? 1 : mass(rank_score(sh.key[i]));
+                __syncthreads();
+                for (int i = threadIdx.x; i < n; i += NT) {
+                    const uint64_t key = sh.key[i];
+                    unsigned long long above = 0;
+                    for (int j = 0; j < n; ++j) above += sh.key[j] > key ? sh.key_mass[j] : 0;
+                    // (a goal of next to nothing still keeps the first label)
+                    if (front + above == 0 || (double)(front + above) < goal) {
+                        atomicMin(&sh.low_key, key);
+                        // (sums of integers: in any order)
+                        if (final && weight(rank_score(key)) >= f.min_p)
+                            atomicAdd(&sh.more[rank_label(key) / (step * per)], (unsigned long long)mass(rank_score(key)));
+                    }
+                }
+                __syncthreads();
+                cut = sh.low_key;
+                if (final) {
+                    for (int i = threadIdx.x; i < count_runs; i += NT) sh.runs[i] += __builtin_ldexp((double)sh.more[i], -bits);
+                    __syncthreads();
+                    summed = true;
+                }
+            } else {
+                // the largest key from which on at least `goal` is held
+                uint64_t best = 0;
+#pragma unroll 1
+                for (int b = 63; b >= 0; --b) {
+                    const uint64_t at = best | 1ull << b, from = at > cut ? at : cut;
+                    unsigned long long held = 0;
+                    each([&](float x, int c) __attribute__((always_inline)) {
+                        if (bin_of(x) == bin && rank_key(score_key(x), c) >= from) held += count ? 1 : mass(x);
+                    });
+                    held = block_sum<unsigned long long, NT>(held, sh.upart);
+                    if (held && (double)(front + held) >= goal) best = at;
+                }
+                cut = best > cut ? best : cut;
+            }
+            if (!final) {
                 // what is left of the bin, and nothing behind it
-                const int bin = bin_of(rank_score(low));
                 unsigned long long left = 0;
-                each([&](float x, int c) {
-                    if (bin_of(x) == bin && rank_key(score_key(x), c) >= low) left += mass(x);
+                each([&](float x, int c) __attribute__((always_inline)) {
+                    if (bin_of(x) == bin && rank_key(score_key(x), c) >= cut) left += mass(x);
                 });
                 left = block_sum<unsigned long long, NT>(left, sh.upart);
                 for (int i = threadIdx.x; i < kBins; i += NT)
@@ -743,34 +891,17 @@ template <typename T, int NT> struct BlockRow {
                 __syncthreads();
             }
         }
-        if (masses) {
-            unsigned long long mine = 0;
-            for (int i = threadIdx.x; i < kBins; i += NT) mine += sh.masses[i];
-            const double total = (double)block_sum<unsigned long long, NT>(mine, sh.upart);
-            const double goal = f.top_p * total;
-            // (nothing to reach: the first label stays alone)
-            low = goal > 0 ? cut_at<false>(goal, low) : cut_at<true>(1.0, 0);
-        }
-        return low;
+        if (!summed) sweep<false>(sure, open, cut, f.min_p);
+        return cut;
     }
 
-    // Step 4.  cut: lowest rank key that stays
-    __device__ void draw(uint64_t cut, double min_p, float u, unsigned r, const Out &out)
+    // Step 4: sh.runs holds the runs' kept weights, cut is the lowest rank key that stays
+    MFL_INLINE void draw(uint64_t cut, double min_p, float u, unsigned r, const Out &out)
     {
-        constexpr int V = kVec<T>, step = 64 * V;
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int tiles = (C + step - 1) / step, per = (tiles + kRuns - 1) / kRuns, runs = (tiles + per - 1) / per;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, runs = count_runs;
         const float cut_score = cut ? rank_score(cut) : -INFINITY;
-        // a tile's kept weights
-        auto tile = [&](int t, double (&w)[V]) {
-            const int c = t * step + lane * V;
-            float x[V];
-            if (sc == 1 && c + V <= C) {
-                load_vec(p + c, x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) x[i] = c + i < C ? to_float(p[(c + i) * sc]) : -INFINITY;
-            }
+        // a vector's kept weights
+        auto kept = [&](const float (&x)[V], int c, double (&w)[V]) {
             float best = x[0];
 #pragma unroll
             for (int i = 1; i < V; ++i) best = fmaxf(best, x[i]);
@@ -785,21 +916,6 @@ template <typename T, int NT> struct BlockRow {
             }
             return some;
         };
-        for (int e = wave; e < runs; e += NT / 64) {
-            double sum = 0;
-            for (int t = e * per; t < min(tiles, (e + 1) * per); ++t) {
-                double w[V];
-                if (!tile(t, w)) continue;
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum += w[i];
-            }
-            if (__any(sum > 0)) {
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-            }
-            if (lane == 0) sh.runs[e] = sum;
-        }
-        __syncthreads();
         // the run that the draw falls into, or the last one that holds something
         constexpr int mine = kRuns / NT > 0 ? kRuns / NT : 1;
         double sum = 0, all;
@@ -834,8 +950,10 @@ template <typename T, int NT> struct BlockRow {
         int label = -1;
         double got = 0;
         for (int t = run * per; t < min(tiles, (run + 1) * per); ++t) {
+            float x[V];
+            load_tile(x, t);
             double w[V];
-            if (!tile(t, w)) continue;
+            if (!kept(x, t * step + lane * V, w)) continue;
             double own = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) own += w[i];
@@ -871,25 +989,209 @@ template <typename T, int NT> struct BlockRow {
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT)
-sample_blocks_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
+sample_blocks_kernel(Rows in, Settings set, int done, const float *__restrict__ uniform, Out out)
 {
     __shared__ typename BlockRow<T, NT>::Shared sh;
     const unsigned r = blockIdx.x;
     const RowOf<T> at(in, r);
     const Filter f = filter_of(set, at.n, in.C);
-    const int wide = 32 - __builtin_clz(in.C);      // C < 2^wide
-    BlockRow<T, NT> row = {sh, at.p, in.sc, in.C, 0.f, 0.f, {}, min(51, 62 - wide)};
+    if (f.top_k <= done) return;            // (a list had it)
+    BlockRow<T, NT> row(sh, at.p, in.sc, in.C);
     row.largest();
     if (!(fabsf(row.m) < INFINITY)) {
         if (threadIdx.x == 0) put(out, r, -1, -INFINITY);
         return;
     }
-    row.scale = (float)fmin(f.inv_t * kBinsPerUnit, 1e30);
-    row.weight = {row.m, f.inv_t * kLog2eD};
-    const uint64_t cut = f.top_k < in.C || f.top_p < 1 ? row.cut(f) : 0;
-    __syncthreads();
+    row.set(f);
+    const uint64_t cut = row.cut_of(f);
     row.draw(cut, f.min_p, uniform[r], r, out);
 }
+
+// ---- rows of many labels without top_k and top_p: cut into parts
+//
+// A workgroup holds a part's scores in registers: the part's largest score, and the weights next to it (with min_p, in a
+// second launch, next to the row's largest), summed.  One workgroup per row then scales the sums, finds the part that the
+// draw falls into, and reads that part again.
+
+constexpr int kPlainThreads = 256;
+constexpr int kPlainPart = 8192;            // labels of a part at most
+struct Part {
+    double sum;
+    float top;
+};
+template <typename T> constexpr int kPlainVecs = kPlainPart / (kPlainThreads * kVec<T>);
+
+// A thread's vectors of a part: labels begin + (u * 256 + thread) * V
+template <typename T> __device__ inline void load_part(float (&x)[kPlainVecs<T>][kVec<T>], const T *p, long long sc, int begin, int end)
+{
+    constexpr int V = kVec<T>, U = kPlainVecs<T>;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = begin + (u * kPlainThreads + (int)threadIdx.x) * V;
+        if (sc == 1 && c + V <= end) {
+            load_vec(p + c, x[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[u][i] = c + i < end ? to_float(p[(c + i) * sc]) : -INFINITY;
+        }
+    }
+}
+__device__ inline float block_largest(float v, float *part)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max_or_nan(v, __shfl_xor(v, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    for (int w = 0; w < kPlainThreads / 64; ++w) v = max_or_nan(v, part[w]);
+    return v;
+}
+// The row's largest score
+__device__ inline float largest_of_parts(const Part *parts, int n, float *part)
+{
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += kPlainThreads) m = max_or_nan(m, parts[i].top);
+    return block_largest(m, part);
+}
+
+template <typename T, bool AGAIN>
+__global__ void __launch_bounds__(kPlainThreads)
+plain_parts_kernel(Rows in, Settings set, int parts, int size, Part *__restrict__ ws)
+{
+    __shared__ float fpart[kPlainThreads / 64];
+    __shared__ double dpart[kPlainThreads / 64];
+    constexpr int V = kVec<T>, U = kPlainVecs<T>;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const RowOf<T> row(in, r);
+    const Filter f = filter_of(set, row.n, in.C);
+    const int begin = part * size, end = min(in.C, begin + size);
+    float x[U][V];
+    load_part(x, row.p, in.sc, begin, end);
+    float m;
+    if (AGAIN) {
+        m = largest_of_parts(ws + (size_t)r * parts, parts, fpart);
+    } else {
+        m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) m = largest_of(x[u], m);
+        m = block_largest(m, fpart);
+    }
+    double sum = 0;
+    if (fabsf(m) < INFINITY) {
+        const Weight weight = {m, f.inv_t * kLog2eD};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (begin + u * kPlainThreads * V >= end) break;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double w = weight(x[u][i]);
+                sum += !AGAIN || w >= f.min_p ? w : 0.0;
+            }
+        }
+    }
+    sum = block_sum<double, kPlainThreads>(sum, dpart);
+    if (threadIdx.x == 0) {
+        ws[blockIdx.x].sum = sum;
+        if (!AGAIN) ws[blockIdx.x].top = m;
+    }
+}
+
+template <typename T, bool AGAIN>
+__global__ void __launch_bounds__(kPlainThreads)
+plain_pick_kernel(Rows in, Settings set, int parts, int size, const Part *__restrict__ ws, const float *__restrict__ uniform, Out out)
+{
+    constexpr int V = kVec<T>, U = kPlainVecs<T>;
+    __shared__ float fpart[kPlainThreads / 64];
+    __shared__ double dpart[kPlainThreads / 64], sums[U * kPlainThreads], before;
+    __shared__ unsigned first, last;
+    const unsigned r = blockIdx.x;
+    const RowOf<T> row(in, r);
+    const Filter f = filter_of(set, row.n, in.C);
+    ws += (size_t)r * parts;
+    const float m = largest_of_parts(ws, parts, fpart);
+    if (!(fabsf(m) < INFINITY)) {
+        if (threadIdx.x == 0) put(out, r, -1, -INFINITY);
+        return;
+    }
+    const Weight weight = {m, f.inv_t * kLog2eD};
+    auto scaled = [&](int i) { return AGAIN ? ws[i].sum : ws[i].sum * weight(ws[i].top); };
+    // the first of n entries whose running sum exceeds the target, or the last that holds something; what lies in front
+    auto find = [&](int n, auto value, double front0, double &target, double &all, bool given) {
+        const int each = (n + kPlainThreads - 1) / kPlainThreads, from = min(n, (int)threadIdx.x * each), to = min(n, from + each);
+        double mine = 0;
+        int holds = -1;
+        for (int i = from; i < to; ++i) {
+            const double v = value(i);
+            mine += v;
+            if (v > 0) holds = i;
+        }
+        double sum, front = front0 + block_front<double, kPlainThreads>(mine, dpart, sum);
+        if (!given) {
+            all = sum;
+            target = draw_of(uniform[r]) * all;
+        }
+        if (threadIdx.x == 0) first = ~0u, last = 0;
+        __syncthreads();
+        if (holds >= 0) atomicMax(&last, (unsigned)holds);
+        if (mine > 0 && front + mine > target) {
+            double run = front;
+            for (int i = from; i < to; ++i) {
+                run += value(i);
+                if (run > target) {
+                    atomicMin(&first, (unsigned)i);
+                    break;
+                }
+            }
+        }
+        __syncthreads();
+        const int at = first != ~0u ? (int)first : (int)last;
+        if (at >= from && at < to) {
+            for (int i = from; i < at; ++i) front += value(i);
+            before = front;
+        }
+        __syncthreads();
+        return at;
+    };
+    double target = 0, total = 0;
+    const int part = find(parts, scaled, 0.0, target, total, false);
+    const double front = before;
+    __syncthreads();
+    const int begin = part * size, end = min(in.C, begin + size);
+    float x[U][V];
+    load_part(x, row.p, in.sc, begin, end);
+    auto kept = [&](float v) {
+        const double w = weight(v);
+        return w >= f.min_p ? w : 0.0;
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        double s = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += kept(x[u][i]);
+        sums[u * kPlainThreads + threadIdx.x] = s;
+    }
+    __syncthreads();
+    const int vec = find(U * kPlainThreads, [&](int i) { return sums[i]; }, front, target, total, true);
+    if (threadIdx.x) return;
+    double run = before, got = 0;
+    int label = -1;
+    for (int c = begin + vec * V; c < min(end, begin + (vec + 1) * V); ++c) {
+        const double w = kept(to_float(row.p[c * in.sc]));
+        if (w == 0) continue;
+        run += w;
+        label = c;
+        got = w;
+        if (run > target) break;
+    }
+    put(out, r, label, log(got / total));
+}
+
+int plain_part_labels(unsigned rows, int C)
+{
+    // a quarter of the full size where that leaves the card short of workgroups
+    return (unsigned long long)rows * ((C + kPlainPart - 1) / kPlainPart) >= 1024 ? kPlainPart : kPlainPart / 4;
+}
+int plain_parts(unsigned rows, int C) { return (int)(((long long)C + plain_part_labels(rows, C) - 1) / plain_part_labels(rows, C)); }
 
 // top_k for all rows, and short enough for a list (temperature 0: the best one)
 int list_length(const Settings &set)
@@ -898,50 +1200,91 @@ int list_length(const Settings &set)
     if (!set.t_n && set.t == 0) return 1;
     return set.top_k >= 1 && set.top_k <= MFL_MAX_TOP_LABELS ? set.top_k : 0;
 }
-bool by_lanes(const Rows &in) { return !(in.sc == 1 && in.C >= 256); }
+
+enum Way { LONE, LANES, LIST_LANES, ANY_LANES, PLAIN, WAVES, BLOCKS };
+struct Plan {
+    Way way;
+    int k;                      // length of the list, 0: none
+    bool two;                   // WAVES, then BLOCKS for the rows whose own top_k is not that short
+    size_t bytes;
+};
+Plan plan_of(const Rows &in, const Settings &set)
+{
+    const bool no_k = !set.top_k_n && (set.top_k == 0 || set.top_k >= in.C), no_p = !set.top_p_n && set.top_p == 1;
+    const bool plain = no_k && no_p && !set.t_n && set.t > 0 && !set.min_p_n;
+    const int k = list_length(set) < in.C ? list_length(set) : 0;
+    const auto keys = [&](int k) {
+        const int parts = row_per_wave(in.rows, in.C) ? 1 : top_parts(in.rows, in.C);
+        return parts > 1 ? (size_t)in.rows * parts * part_keys(k) * sizeof(uint64_t) : 0;
+    };
+    // lanes: short rows, and planes of many rows
+    if (!(in.sc == 1 && in.C >= 256) && !(in.C >= 1024 && in.rows <= 4096)) {
+        const int list = k ? k : no_k && in.C <= 32 ? in.C : 0;
+        if (plain) return {in.C <= kLoneBlock ? LONE : LANES, 0, false, 0};
+        if (list && list <= 32 && in.C <= kBestLabels) return {LIST_LANES, list, false, 0};
+        // (a lane that has to search for its cut takes longer than a workgroup; from here on there are enough lanes)
+        if (in.rows > 16384) return {ANY_LANES, 0, false, 0};
+    }
+    if (plain && in.C > 4096) return {PLAIN, 0, false, (size_t)in.rows * plain_parts(in.rows, in.C) * sizeof(Part)};
+    if (k) return {WAVES, k, false, keys(k)};
+    if (set.top_k_n && in.C > MFL_MAX_TOP_LABELS) return {WAVES, MFL_MAX_TOP_LABELS, true, keys(MFL_MAX_TOP_LABELS)};
+    return {BLOCKS, 0, false, 0};
+}
 
 template <typename T>
 int run(const Rows &in, const Settings &set, const float *uniform, const Out &out, void *workspace, hipStream_t st)
 {
-    if (by_lanes(in)) {
-        const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
+    const Plan plan = plan_of(in, set);
+    const int k = plan.k;
+    const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
 #define MFL_LANES(...) hipLaunchKernelGGL(__VA_ARGS__, grid, block, 0, st, in, set, uniform, out)
-        // what the list has to hold: top_k, or with top_p alone every label
-        const bool no_k = !set.top_k_n && (set.top_k == 0 || set.top_k >= in.C), no_p = !set.top_p_n && set.top_p == 1;
-        const bool same_t = !set.t_n && set.t > 0, below_1 = !set.min_p_n;
-        const int k = list_length(set) ? list_length(set) : no_k && in.C <= 32 ? in.C : 0;
-        if (no_k && no_p && same_t && below_1) {
-            if (in.C <= 8) MFL_LANES((plain_lone_kernel<T, 8>));
-            else if (in.C <= kLoneBlock) MFL_LANES((plain_lone_kernel<T, kLoneBlock>));
-            else MFL_LANES((plain_lanes_kernel<T>));
-        } else if (k && k <= 32 && in.C <= kBestLabels) {
-            if (k <= 1) MFL_LANES((list_lanes_kernel<T, 1>));
-            else if (k <= 4) MFL_LANES((list_lanes_kernel<T, 4>));
-            else if (k <= 8) MFL_LANES((list_lanes_kernel<T, 8>));
-            else if (k <= 16) MFL_LANES((list_lanes_kernel<T, 16>));
-            else if (k <= 24) MFL_LANES((list_lanes_kernel<T, 24>));
-            else MFL_LANES((list_lanes_kernel<T, 32>));
-        } else {
-            MFL_LANES((any_lanes_kernel<T>));
-        }
+    switch (plan.way) {
+    case LONE:
+        if (in.C <= 8) MFL_LANES((plain_lone_kernel<T, 8>));
+        else MFL_LANES((plain_lone_kernel<T, kLoneBlock>));
+        break;
+    case LANES: MFL_LANES((plain_lanes_kernel<T>)); break;
+    case LIST_LANES:
+        if (k <= 1) MFL_LANES((list_lanes_kernel<T, 1>));
+        else if (k <= 4) MFL_LANES((list_lanes_kernel<T, 4>));
+        else if (k <= 8) MFL_LANES((list_lanes_kernel<T, 8>));
+        else if (k <= 16) MFL_LANES((list_lanes_kernel<T, 16>));
+        else if (k <= 24) MFL_LANES((list_lanes_kernel<T, 24>));
+        else MFL_LANES((list_lanes_kernel<T, 32>));
+        break;
+    case ANY_LANES: MFL_LANES((any_lanes_kernel<T>)); break;
 #undef MFL_LANES
-        return (int)hipGetLastError();
+    case PLAIN: {
+        const int parts = plain_parts(in.rows, in.C), size = plain_part_labels(in.rows, in.C);
+        Part *ws = (Part *)workspace;
+        const dim3 all(in.rows * parts), one(in.rows), threads(kPlainThreads);
+        hipLaunchKernelGGL((plain_parts_kernel<T, false>), all, threads, 0, st, in, set, parts, size, ws);
+        if (set.min_p > 0) {
+            hipLaunchKernelGGL((plain_parts_kernel<T, true>), all, threads, 0, st, in, set, parts, size, ws);
+            hipLaunchKernelGGL((plain_pick_kernel<T, true>), one, threads, 0, st, in, set, parts, size, ws, uniform, out);
+        } else {
+            hipLaunchKernelGGL((plain_pick_kernel<T, false>), one, threads, 0, st, in, set, parts, size, ws, uniform, out);
+        }
+        break;
     }
-    const int k = list_length(set) < in.C ? list_length(set) : 0;
-    if (k) {
-        if (in.C < kBlockLabels) {
+    case WAVES: {
+        if (row_per_wave(in.rows, in.C)) {
             const unsigned per = kWaveTopThreads / 64;
             hipLaunchKernelGGL(list_waves_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kWaveTopThreads), 0, st, in, set, k, uniform, out);
-            return (int)hipGetLastError();
+        } else {
+            const int parts = top_parts(in.rows, in.C);
+            uint64_t *keys = (uint64_t *)workspace;
+            hipLaunchKernelGGL(list_parts_kernel<T>, dim3(in.rows * parts), dim3(kWaveTopThreads), 0, st, in, set, k, parts, uniform, keys, out);
+            if (parts > 1)
+                hipLaunchKernelGGL(list_join_kernel, dim3(in.rows), dim3(kWaveTopThreads), 0, st, in, set, k, parts, uniform, keys, out);
         }
-        const int parts = top_parts(in.rows, in.C);
-        uint64_t *keys = (uint64_t *)workspace;
-        hipLaunchKernelGGL(list_parts_kernel<T>, dim3(in.rows * parts), dim3(kWaveTopThreads), 0, st, in, set, k, parts, uniform, keys, out);
-        if (parts > 1) hipLaunchKernelGGL(list_join_kernel<T>, dim3(in.rows), dim3(64), 0, st, in, set, k, parts, uniform, keys, out);
-        return (int)hipGetLastError();
+        if (!plan.two) break;
+        [[fallthrough]];
     }
-    if (in.C <= 4096) hipLaunchKernelGGL((sample_blocks_kernel<T, 256>), dim3(in.rows), dim3(256), 0, st, in, set, uniform, out);
-    else hipLaunchKernelGGL((sample_blocks_kernel<T, 1024>), dim3(in.rows), dim3(1024), 0, st, in, set, uniform, out);
+    case BLOCKS:
+        if (in.C <= 4096) hipLaunchKernelGGL((sample_blocks_kernel<T, 256>), dim3(in.rows), dim3(256), 0, st, in, set, k, uniform, out);
+        else hipLaunchKernelGGL((sample_blocks_kernel<T, 1024>), dim3(in.rows), dim3(1024), 0, st, in, set, k, uniform, out);
+    }
     return (int)hipGetLastError();
 }
 
@@ -949,12 +1292,19 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
 
 extern "C" {
 
+// (for any strides and settings: the most that a call of this size takes)
 size_t mfl_sample_labels_workspace_bytes(int N, int C, int S, int dtype)
 {
     Rows in;
-    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || C < kBlockLabels) return 0;
-    const int parts = top_parts(in.rows, in.C);
-    return parts > 1 ? (size_t)in.rows * parts * MFL_MAX_TOP_LABELS * sizeof(uint64_t) : 0;
+    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0)) return 0;
+    size_t most = 0;
+    const Settings sets[2] = {{1.0, 1.0, 0.0, 0, nullptr, nullptr, nullptr, nullptr}, {1.0, 1.0, 0.0, MFL_MAX_TOP_LABELS, nullptr, nullptr, nullptr, nullptr}};
+    for (int i = 0; i < 4; ++i) {
+        in.sc = i & 1 ? 1 : 2;
+        const size_t n = plan_of(in, sets[i >> 1]).bytes;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 int mfl_sample_labels(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c, long long stride_s,
@@ -971,9 +1321,9 @@ int mfl_sample_labels(const void *scores, int dtype, int N, int C, int S, long l
     if ((!temperature_n && temperature != 0 && !temperature_ok(temperature)) || (!top_k_n && top_k < 0) ||
         (!top_p_n && !(top_p > 0 && top_p <= 1)) || (!min_p_n && !(min_p >= 0 && min_p <= 1)))
         return MFL_ERR_INVALID_ARGUMENT;
-    const size_t need = by_lanes(in) ? 0 : mfl_sample_labels_workspace_bytes(N, C, S, dtype);
-    if (need && (!workspace || workspace_bytes < need)) return MFL_ERR_WORKSPACE;
     const Settings set = {temperature, top_p, min_p, top_k, temperature_n, top_p_n, min_p_n, top_k_n};
+    const size_t need = plan_of(in, set).bytes;
+    if (need && (!workspace || workspace_bytes < need)) return MFL_ERR_WORKSPACE;
     const Out out = {labels, label_bytes, logprob};
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {

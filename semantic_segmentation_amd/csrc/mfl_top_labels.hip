@@ -63,7 +63,7 @@ top_lanes_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, 
 }
 
 template <typename T>
-__device__ inline void put_row(const WaveTop<true> &top, const Rows &in, unsigned r, int k, float inv_t, T *values, int *labels, float *rest)
+__device__ inline void put_row(WaveTop<true> &top, const Rows &in, unsigned r, int k, float inv_t, T *values, int *labels, float *rest)
 {
     const unsigned n = r / in.S, s = r - n * in.S;
     const size_t base = (size_t)n * k * in.S + s;
@@ -113,39 +113,45 @@ top_parts_kernel(Rows in, float c2, float inv_t, int k, int parts, uint64_t *__r
     const int begin = min(in.C, (int)part * size), end = min(in.C, begin + size);
     if (!top_of_part(top, sh, p, in.sc, begin, end)) return;
     if (parts == 1) {
+        top.cut();
         put_row(top, in, r, k, inv_t, values, labels, rest);
         return;
     }
-    for (int j = lane; j < k; j += 64) keys[(size_t)blockIdx.x * k + j] = j < top.count ? top.list[j] : 0;
+    const int slots = part_keys(k);
+    for (int j = lane; j < slots; j += 64) keys[(size_t)blockIdx.x * slots + j] = j < top.count ? top.list[j] : 0;
     const LogSum sum = wave_join(top.rest, c2);
     if (lane == 0) sums[blockIdx.x] = sum;
 }
 
-// One wave per row: the best of its parts' best
+// One workgroup per row: the best of its parts' best
 template <typename T>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(kWaveTopThreads)
 top_join_kernel(Rows in, float c2, float inv_t, int k, int parts, const uint64_t *__restrict__ keys, const LogSum *__restrict__ sums,
                 T *__restrict__ values, int *__restrict__ labels, float *__restrict__ rest)
 {
-    __shared__ uint64_t list[kListKeys];
-    const int lane = threadIdx.x;
+    __shared__ TopShared sh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned r = blockIdx.x;
-    WaveTop<true> top(list, k, c2);
-    top.join(keys + (size_t)r * parts * k, parts * k);
+    const int n = parts * part_keys(k);
+    WaveTop<true> top(sh.lists[wave], k, c2);
+    if (!top_of_keys(top, sh, keys + (size_t)r * n, n)) return;
     top.cut();
-    for (int i = lane; i < parts; i += 64) top.rest = join(top.rest, sums[(size_t)r * parts + i], c2);
+    if (lane < parts) top.rest = join(top.rest, sums[(size_t)r * parts + lane], c2);
     put_row(top, in, r, k, inv_t, values, labels, rest);
 }
 
 // Rows of many neighbouring labels, long lists, and few rows go to waves
-bool by_waves(const Rows &in, int k) { return k > 32 || in.C > kBestLabels || in.rows < 64 || (in.sc == 1 && in.C >= 256); }
+bool by_waves(const Rows &in, int k)
+{
+    return k > 32 || in.C > kBestLabels || (in.sc == 1 && in.C >= 256) || (in.C >= 1024 && in.rows <= 4096);
+}
 
 template <typename T>
 int run(const Rows &in, double temperature, int k, void *values, int *labels, float *rest, void *workspace, hipStream_t st)
 {
     const float c2 = (float)(kLog2eD / temperature), inv_t = (float)(1.0 / temperature);
     if (by_waves(in, k)) {
-        if (in.C < kBlockLabels) {
+        if (row_per_wave(in.rows, in.C)) {
             const unsigned per = kWaveTopThreads / 64;
             hipLaunchKernelGGL(top_waves_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k,
                                (T *)values, labels, rest);
@@ -153,11 +159,11 @@ int run(const Rows &in, double temperature, int k, void *values, int *labels, fl
         }
         const int parts = top_parts(in.rows, in.C);
         uint64_t *keys = (uint64_t *)workspace;
-        LogSum *sums = (LogSum *)(keys + (size_t)in.rows * parts * k);
+        LogSum *sums = (LogSum *)(keys + (size_t)in.rows * parts * part_keys(k));
         hipLaunchKernelGGL(top_parts_kernel<T>, dim3(in.rows * parts), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k, parts, keys, sums,
                            (T *)values, labels, rest);
         if (parts > 1)
-            hipLaunchKernelGGL(top_join_kernel<T>, dim3(in.rows), dim3(64), 0, st, in, c2, inv_t, k, parts, keys, sums, (T *)values, labels,
+            hipLaunchKernelGGL(top_join_kernel<T>, dim3(in.rows), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k, parts, keys, sums, (T *)values, labels,
                                rest);
         return (int)hipGetLastError();
     }
@@ -182,7 +188,7 @@ size_t mfl_top_labels_workspace_bytes(int N, int C, int S, int dtype, int k)
     Rows in;
     if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || k < 1 || k > MFL_MAX_TOP_LABELS) return 0;
     const int parts = top_parts(in.rows, in.C);
-    return parts > 1 ? (size_t)in.rows * parts * (k * sizeof(uint64_t) + sizeof(LogSum)) : 0;
+    return parts > 1 ? (size_t)in.rows * parts * (part_keys(k) * sizeof(uint64_t) + sizeof(LogSum)) : 0;
 }
 
 int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c, long long stride_s,

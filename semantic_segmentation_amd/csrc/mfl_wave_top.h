@@ -18,6 +18,9 @@ namespace mfl_scores {
 constexpr int kWaveTopThreads = 256;
 constexpr int kListKeys = 1024;
 
+// Keys a search leaves at most, and a part of a row hands on
+__host__ __device__ inline int part_keys(int k) { return k < 64 ? 2 * k + 32 : k + k / 2; }
+
 typedef __attribute__((address_space(3))) uint64_t lds_key;
 
 template <bool REST> struct WaveTop {
@@ -110,7 +113,7 @@ template <bool REST> struct WaveTop {
         bound_score = rank_score(bound);
         __builtin_amdgcn_wave_barrier();
     }
-    __device__ int most() const { return k < 64 ? 2 * k + 32 : k + k / 2; }
+    __device__ int most() const { return part_keys(k); }
 
     // Keeps the list short: its bound is only as tight as the last search
     __device__ void room()
@@ -171,7 +174,8 @@ template <bool REST> struct WaveTop {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int u = 0; u < 4; ++u) m[u] = -INFINITY;
-        for (int v = 0; v < vectors; v += 4) {
+        int v = 0;
+        for (; v + 4 <= vectors; v += 4) {
             float x[4][V];
 #pragma unroll
             for (int u = 0; u < 4; ++u) load_vec(p + begin + ((v + u) * 64 + lane) * V, x[u]);
@@ -179,6 +183,12 @@ template <bool REST> struct WaveTop {
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < V; ++i) m[u] = fmaxf(m[u], x[u][i]);
+        }
+        for (; v < vectors; ++v) {
+            float x[V];
+            load_vec(p + begin + (v * 64 + lane) * V, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) m[0] = fmaxf(m[0], x[i]);
         }
     }
     // A bound to begin with, from the largest scores of 256 disjoint sets of labels, four a lane: where k sets hold a score
@@ -250,23 +260,31 @@ template <bool REST> struct WaveTop {
     template <typename Key> __device__ void join(Key *keys, int n)
     {
         const int lane = threadIdx.x & 63;
+        if (n <= 0) return;
+        auto ahead = [&](int i) { return (uint64_t)keys[min(i + lane, n - 1)]; };
+        uint64_t next[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) next[u] = ahead(64 * u);
 #pragma unroll 1
         for (int i = 0; i < n; i += 64) {
-            const uint64_t key = i + lane < n ? keys[i + lane] : 0;
+            const uint64_t key = i + lane < n ? next[0] : 0;
+#pragma unroll
+            for (int u = 0; u < 3; ++u) next[u] = next[u + 1];
+            next[3] = ahead(i + 4 * 64);
             room();
             const bool in = append(key, key != 0);
-            if (REST && !in && key) add_score(rest, rank_score(key), c2);
+            if (REST && __any(!in && key)) add_score(rest, !in && key ? rank_score(key) : -INFINITY, c2);
         }
     }
 
-    // Down to the k best
+    // Down to at most as many as ranked() and a draw take
     __device__ void cut()
     {
-        if (count > k) shrink(k, k);
+        if (count > MFL_MAX_TOP_LABELS) shrink(k, MFL_MAX_TOP_LABELS);
     }
 
-    // f(rank, key) for each of the list's keys (at most 128), by counting what is above it
-    template <typename F> __device__ void ranked(F f) const
+    // f(rank, key) for the k best of at most 128 keys, by counting what is above each; the others go to the rest
+    template <typename F> __device__ void ranked(F f)
     {
         const int lane = threadIdx.x & 63;
         __builtin_amdgcn_wave_barrier();
@@ -277,16 +295,18 @@ template <bool REST> struct WaveTop {
             above_a += key > a;
             above_b += key > b;
         }
-        if (a) f(above_a, a);
-        if (b) f(above_b, b);
+        if (a && above_a < k) f(above_a, a);
+        if (b && above_b < k) f(above_b, b);
+        const float out[2] = {a && above_a >= k ? rank_score(a) : -INFINITY, b && above_b >= k ? rank_score(b) : -INFINITY};
+        if (REST) add_to_rest(out);
     }
 };
 
 // ---- a workgroup's four waves on one part of a row, or on four rows
 //
-// Four waves on one part agree on the bound to begin with: each brings the largest scores of 64 sets of 64 labels or so, and
-// with k = 64 of 256 sets the bound lets 0.5 % of scores in random order through, an eighth of what a wave's own look at
-// 16 labels a set would.  The first wave then joins the four lists.
+// Four waves on one part agree on the bound to begin with: every lane brings the largest of up to 64 scores.  At k = 64 of 256
+// such sets the bound lets 0.5 % of scores in random order through, where a wave's own look lets 1.8 % through.  The first
+// wave then joins the four lists.
 
 struct TopShared {
     uint64_t lists[kWaveTopThreads / 64][kListKeys];
@@ -295,26 +315,11 @@ struct TopShared {
     int count[kWaveTopThreads / 64];
 };
 
-// After it the first wave's list holds the part's k best and its lanes the shares of the rest; the other waves are done.
-template <bool REST, typename T>
-__device__ inline bool top_of_part(WaveTop<REST> &top, TopShared &sh, const T *p, long long sc, int begin, int end)
+// The first wave takes over the four lists.  After it its list holds the part's k best and perhaps more (no more than
+// most()), and its lanes the shares of the rest; the other waves are done (false).
+template <bool REST> __device__ inline bool join_waves(WaveTop<REST> &top, TopShared &sh)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int step = 64 * kVec<T>;
-    const int quarter = ((end - begin + 3) / 4 + step - 1) / step * step;
-    const int from = min(end, begin + wave * quarter), to = min(end, from + quarter);
-    // (every wave has the vectors to look at, and they are at most half of what there is)
-    const int vectors = sc == 1 && end - begin - 3 * quarter >= 8 * step ? (quarter >= 16 * step ? 8 : 4) : 0;
-    if (vectors) {
-        float m[4];
-        WaveTop<REST>::look(p, from, vectors, m);
-        sh.seen[threadIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 4; ++u) m[u] = sh.seen[lane + 64 * u];
-        top.foresee(m);
-    }
-    top.stream(p, sc, from, to);
     if (top.count > kListKeys / 2) top.shrink(top.k, top.most());
     const LogSum rest = wave_join(top.rest, top.c2);
     if (lane == 0) {
@@ -327,21 +332,67 @@ __device__ inline bool top_of_part(WaveTop<REST> &top, TopShared &sh, const T *p
         top.join((lds_key *)sh.lists[w], sh.count[w]);
         if (REST && lane == 0) top.rest = join(top.rest, sh.rest[w], top.c2);
     }
-    top.cut();
+    if (top.count > top.most()) top.shrink(top.k, top.most());
     return true;
 }
+// Every lane brings the largest score it has seen
+template <bool REST> __device__ inline void agree(WaveTop<REST> &top, TopShared &sh, float seen)
+{
+    const int lane = threadIdx.x & 63;
+    sh.seen[threadIdx.x] = seen;
+    __syncthreads();
+    float m[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) m[u] = sh.seen[lane + 64 * u];
+    top.foresee(m);
+}
 
-// Labels from which on a part gets a whole workgroup
-constexpr int kBlockLabels = 8192;
+template <bool REST, typename T>
+__device__ inline bool top_of_part(WaveTop<REST> &top, TopShared &sh, const T *p, long long sc, int begin, int end)
+{
+    const int wave = threadIdx.x >> 6;
+    constexpr int step = 64 * kVec<T>;
+    // three waves take whole steps, the last one what is left
+    const int even = (end - begin) / 4 / step * step, quarter = even ? even : step;
+    const int from = min(end, begin + wave * quarter), to = wave == 3 ? end : min(end, from + quarter);
+    if (sc == 1 && even) {
+        float m[4];
+        WaveTop<REST>::look(p, from, min(even / step, 8), m);
+        agree(top, sh, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+    }
+    top.stream(p, sc, from, to);
+    return join_waves(top, sh);
+}
 
-// Parts a row is cut into: enough workgroups for the card, at least kBlockLabels labels each
+// ... of the keys that parts of a row left (0: none)
+template <bool REST> __device__ inline bool top_of_keys(WaveTop<REST> &top, TopShared &sh, const uint64_t *keys, int n)
+{
+    uint64_t best = 0;
+    for (int i = threadIdx.x; i < n; i += 8 * kWaveTopThreads) {
+        uint64_t key[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) key[u] = i + u * kWaveTopThreads < n ? keys[i + u * kWaveTopThreads] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) best = key[u] > best ? key[u] : best;
+    }
+    agree(top, sh, best ? rank_score(best) : -INFINITY);
+    const int wave = threadIdx.x >> 6, quarter = (n + 3) / 4;
+    const int from = min(n, wave * quarter), to = min(n, from + quarter);
+    top.join(keys + from, to - from);
+    return join_waves(top, sh);
+}
+
+// Parts a row is cut into: enough workgroups for the card (four on each of 256 CUs), at least kPartLabels labels each
+constexpr int kPartLabels = 2048;
 __host__ __device__ inline int top_part_labels(int C, int parts) { return (((C + parts - 1) / parts) + 511) & ~511; }
 inline int top_parts(unsigned rows, int C)
 {
-    const unsigned most = (unsigned)(C / kBlockLabels), want = (1024 + rows - 1) / rows;
+    const unsigned most = (unsigned)(C / kPartLabels), want = (1024 + rows - 1) / rows;
     const unsigned n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
 }
+// One wave per row does where rows are short, or many and not long
+inline bool row_per_wave(unsigned rows, int C) { return C < kPartLabels || (C < 8192 && rows > 1024); }
 
 }  // namespace mfl_scores
 
