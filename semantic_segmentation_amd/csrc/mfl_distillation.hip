@@ -622,7 +622,8 @@ backward_rows_kernel(Rows in, Teacher t, int parts, const float *__restrict__ st
     }
 }
 
-bool by_rows(const Rows &in) { return in.sc == 1 && in.C >= 512; }
+// (few short rows as well: a lane alone takes its time over a long record)
+bool by_rows(const Rows &in) { return in.sc == 1 && (in.C >= 512 || (in.C >= 64 && in.rows <= 16384)); }
 size_t mark_bytes(int C, int parts)
 {
     const int size = part_labels(C, parts);
@@ -701,7 +702,7 @@ extern "C" {
 size_t mfl_distillation_workspace_bytes(int N, int C, int S, int dtype, int k)
 {
     Rows in;
-    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || k < 1 || C < 512) return 0;
+    if (make_rows(in, "", dtype, N, C, S, 0, 1, 0) || k < 1 || !by_rows(in)) return 0;
     return (size_t)in.rows * parts_of(in, kEnough) * sizeof(LogSum);
 }
 

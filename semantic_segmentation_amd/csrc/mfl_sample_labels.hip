@@ -81,7 +81,7 @@ template <typename T> struct RowOf {
 // Without top_k and top_p the labels are streamed once, in blocks: a block's weights next to its own largest score, summed;
 // at the end the block sums are put on one scale, the draw names a block, and that block is read again for the label.  With
 // top_k or top_p the lane keeps its best labels (Best), and looks for the draw among them; where top_p needs more labels than
-// the list holds, a binary search over the rank keys finds the cut.
+// the list holds, it goes on with the next best.
 
 constexpr int kLaneThreads = 256;
 constexpr int kLoneBlock = 24;          // up to this many labels a lane's scores stay in registers
@@ -242,114 +242,26 @@ plain_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out
     plain_lane(in, row.p, filter_of(set, row.n, in.C), uniform[r], r, out, sh);
 }
 
-// The cut by a binary search over the rank keys, then the draw: for any settings
-template <typename T>
-__device__ inline void search_lane(const Rows &in, const T *p, const Filter &f, float u, unsigned r, const Out &out)
+// Takes one block after another into the list: the best labels of those placed before `last`
+template <typename T, int K, typename F> __device__ inline void list_pass(Best<K> &best, const Rows &in, const T *p, double last, F seen)
 {
-    int mk = (int)0x80000000;
-    for (int c = 0; c < in.C; ++c) mk = max(mk, score_key(to_float(p[c * in.sc])));
-    const float m = key_score(mk);
-    if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
-    const Weight weight = {m, f.inv_t * kLog2eD};
-    auto search = [&](auto reached) {
-        uint64_t k = 0;
-        for (int b = 63; b >= 0; --b)
-            if (reached(k | 1ull << b)) k |= 1ull << b;
-        return k;
-    };
-    uint64_t cut = 0;                               // kept by rank: rank_key >= cut
-    if (f.top_k < in.C)
-        cut = search([&](uint64_t k) {
-            int count = 0;
-            for (int c = 0; c < in.C; ++c) count += rank_key(score_key(to_float(p[c * in.sc])), c) >= k;
-            return count >= f.top_k;
-        });
-    if (f.top_p < 1) {
-        auto mass = [&](uint64_t from) {
-            double sum = 0;
-            for (int c = 0; c < in.C; ++c) {
-                const float x = to_float(p[c * in.sc]);
-                if (rank_key(score_key(x), c) >= from) sum += weight(x);
-            }
-            return sum;
-        };
-        const double goal = f.top_p * mass(cut);
-        const uint64_t nucleus = search([&](uint64_t k) {
-            const double sum = mass(k > cut ? k : cut);
-            return sum > 0 && sum >= goal;
-        });
-        cut = nucleus > cut ? nucleus : cut;
-    }
-    auto kept_weight = [&](float x, int c) {
-        const double w = weight(x);
-        return w >= f.min_p && rank_key(score_key(x), c) >= cut ? w : 0.0;
-    };
-    double total = 0;
-    for (int c = 0; c < in.C; ++c) total += kept_weight(to_float(p[c * in.sc]), c);
-    const double target = draw_of(u) * total;
-    double run = 0, got = 0;
-    int label = -1;
-    for (int c = 0; c < in.C; ++c) {
-        const double w = kept_weight(to_float(p[c * in.sc]), c);
-        if (w == 0) continue;
-        run += w;
-        label = c;
-        got = w;
-        if (run > target) break;
-    }
-    put(out, r, label, log(got / total));
-}
-
-// The K best of the row; MASS: also what all labels weigh, for a top_p of more than the list.  Returns false where the list
-// does not reach.
-template <typename T, int K, bool MASS>
-__device__ inline bool list_lane(const Rows &in, const T *p, const Filter &f, float u, unsigned r, const Out &out)
-{
-    Best<K> best;
     constexpr int U = 8;
-    const double a = f.inv_t * kLog2eD;
-    double mass = 0;
-    float m = -INFINITY;
     for (int c = 0; c < in.C; c += U) {
         float x[U];
         load_block(x, p, in.sc, c, in.C);
-        if (MASS) {
-            const float next = largest_of(x, m);
-            if (next != m) mass = m == -INFINITY ? 0.0 : mass * Weight{next, a}(m);
-            m = next;
-            if (m > -INFINITY) {
-                const Weight weight = {m, a};
+        seen(x);
 #pragma unroll
-                for (int i = 0; i < U; ++i) mass += weight(x[i]);
-            }
+        for (int i = 0; i < U; ++i) {
+            const double v = place_of(x[i], c + i);
+            best.insert(c + i < in.C && v < last ? v : 0.0);
         }
-        // (behind the last label: the lowest place of all, below every label's)
-#pragma unroll
-        for (int i = 0; i < U; ++i) best.insert(c + i < in.C ? place_of(x[i], c + i) : 0.0);
     }
-    m = place_score(best.v[0]);
-    if (!(fabsf(m) < INFINITY)) {
-        put(out, r, -1, -INFINITY);
-        return true;
-    }
-    const Weight weight = {m, a};
-    double w[K], total = 0;
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-        w[j] = j < f.top_k && best.v[j] != 0.0 ? weight(place_score(best.v[j])) : 0.0;
-        total += w[j];
-    }
-    if (MASS && f.top_k > K) total = mass;
-    const double goal = f.top_p * total;
-    double front = 0, sum = 0;
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-        const bool keep = j == 0 || ((f.top_p >= 1 || front < goal) && w[j] >= f.min_p);
-        front += w[j];
-        w[j] = keep ? w[j] : 0.0;
-        sum += w[j];
-    }
-    if (MASS && f.top_k > K && in.C > K && (f.top_p >= 1 || front < goal)) return false;
+}
+constexpr double kBeforeAll = 2.0;
+
+// The draw among the list's first labels: w holds what each keeps, sum all of it
+template <int K> __device__ inline void draw_by_label(const Best<K> &best, const double (&w)[K], double sum, float u, unsigned r, const Out &out)
+{
     // label by label, in label order, until the running sum is past the target
     const double target = draw_of(u) * sum;
     double run = 0, got = 0;
@@ -371,9 +283,9 @@ __device__ inline bool list_lane(const Rows &in, const T *p, const Filter &f, fl
         if (run > target) break;
     }
     put(out, r, label, log(got / sum));
-    return true;
 }
 
+// The list holds all that top_k leaves, or all labels
 template <typename T, int K>
 __global__ void __launch_bounds__(kLaneThreads)
 list_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
@@ -381,11 +293,126 @@ list_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out 
     const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
     if (r >= in.rows) return;
     const RowOf<T> row(in, r);
-    list_lane<T, K, false>(in, row.p, filter_of(set, row.n, in.C), uniform[r], r, out);
+    const Filter f = filter_of(set, row.n, in.C);
+    const float u = uniform[r];
+    Best<K> best;
+    list_pass(best, in, row.p, kBeforeAll, [](const float (&)[8]) {});
+    const float m = place_score(best.v[0]);
+    if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
+    const Weight weight = {m, f.inv_t * kLog2eD};
+    double w[K], total = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        w[j] = j < f.top_k && best.v[j] != 0.0 ? weight(place_score(best.v[j])) : 0.0;
+        total += w[j];
+    }
+    const double goal = f.top_p * total;
+    double front = 0, sum = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const bool keep = j == 0 || ((f.top_p >= 1 || front < goal) && w[j] >= f.min_p);
+        front += w[j];
+        w[j] = keep ? w[j] : 0.0;
+        sum += w[j];
+    }
+    draw_by_label(best, w, sum, u, r, out);
 }
 
-// Any settings, of each n its own
-constexpr int kAnyList = 16;
+// Any settings, of each n its own: the best K labels, then the next K, until the cut is found
+template <typename T>
+__device__ inline void ranked_lane(const Rows &in, const T *p, const Filter &f, float u, unsigned r, const Out &out)
+{
+    constexpr int K = 24;
+    const double a = f.inv_t * kLog2eD;
+    double mass = 0;            // of all labels
+    float m = -INFINITY;
+    Best<K> best;
+    list_pass(best, in, p, kBeforeAll, [&](const float (&x)[8]) {
+        const float next = largest_of(x, m);
+        if (next != m) mass = m == -INFINITY ? 0.0 : mass * Weight{next, a}(m);
+        m = next;
+        if (m > -INFINITY && f.top_p < 1 && f.top_k >= in.C) {
+            const Weight weight = {m, a};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mass += weight(x[i]);
+        }
+    });
+    if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
+    const Weight weight = {m, a};
+    // goes on from the list in hand: stop(place, weight, rank) for one label after the other
+    auto in_order = [&](auto stop) {
+        int rank = 0;
+        for (;;) {
+            double last = 0;
+            bool done = false;
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (done || best.v[j] == 0.0) {
+                    done = true;
+                    continue;
+                }
+                last = best.v[j];
+                done = stop(best.v[j], weight(place_score(best.v[j])), rank);
+                ++rank;
+            }
+            if (done || rank >= in.C) return;
+            best = Best<K>();
+            list_pass(best, in, p, last, [](const float (&)[8]) {});
+        }
+    };
+    const Best<K> first = best;
+    double total = mass;
+    if (f.top_p < 1 && f.top_k < in.C) {
+        total = 0;
+        in_order([&](double, double w, int rank) {
+            total += w;
+            return rank + 1 >= f.top_k;
+        });
+        best = first;
+    }
+    const double goal = f.top_p * total;
+    double front = 0, cut = 0;
+    in_order([&](double place, double w, int rank) {
+        if (rank > 0 && (rank >= f.top_k || (f.top_p < 1 && !(front < goal)))) return true;
+        cut = place;
+        front += w;
+        return false;
+    });
+    double sum = 0;
+    auto kept = [&](const float (&x)[8], int c, double (&w)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double v = weight(x[i]);
+            w[i] = c + i < in.C && v >= f.min_p && place_of(x[i], c + i) >= cut ? v : 0.0;
+        }
+    };
+    for (int c = 0; c < in.C; c += 8) {
+        float x[8];
+        double w[8];
+        load_block(x, p, in.sc, c, in.C);
+        kept(x, c, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += w[i];
+    }
+    const double target = draw_of(u) * sum;
+    double run = 0, got = 0;
+    int label = -1;
+    for (int c = 0; c < in.C; c += 8) {
+        float x[8];
+        double w[8];
+        load_block(x, p, in.sc, c, in.C);
+        kept(x, c, w);
+        int here = -1;
+        double v = 0;
+        pick(w, run, target, here, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) run += w[i];
+        if (here >= 0) label = c + here, got = v;
+        if (here >= 0 && run > target) break;
+    }
+    put(out, r, label, log(got / sum));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLaneThreads)
 any_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
@@ -397,8 +424,7 @@ any_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out o
     const Filter f = filter_of(set, row.n, in.C);
     const float u = uniform[r];
     if (f.top_k >= in.C && f.top_p >= 1) return plain_lane(in, row.p, f, u, r, out, sh);
-    if (in.C <= kBestLabels && (f.top_k <= kAnyList || f.top_k >= in.C) && list_lane<T, kAnyList, true>(in, row.p, f, u, r, out)) return;
-    search_lane(in, row.p, f, u, r, out);
+    ranked_lane(in, row.p, f, u, r, out);
 }
 
 // ---- rows that top_k cuts to a short list: of at most k labels (rows of a longer one are passed over)
@@ -1222,8 +1248,8 @@ Plan plan_of(const Rows &in, const Settings &set)
         const int list = k ? k : no_k && in.C <= 32 ? in.C : 0;
         if (plain) return {in.C <= kLoneBlock ? LONE : LANES, 0, false, 0};
         if (list && list <= 32 && in.C <= kBestLabels) return {LIST_LANES, list, false, 0};
-        // (a lane that has to search for its cut takes longer than a workgroup; from here on there are enough lanes)
-        if (in.rows > 16384) return {ANY_LANES, 0, false, 0};
+        // (few rows of many labels to rank: a workgroup each)
+        if (in.C <= kBestLabels && (in.rows > 2048 || in.C <= 64)) return {ANY_LANES, 0, false, 0};
     }
     if (plain && in.C > 4096) return {PLAIN, 0, false, (size_t)in.rows * plain_parts(in.rows, in.C) * sizeof(Part)};
     if (k) return {WAVES, k, false, keys(k)};

@@ -143,7 +143,7 @@ top_join_kernel(Rows in, float c2, float inv_t, int k, int parts, const uint64_t
 // Rows of many neighbouring labels, long lists, and few rows go to waves
 bool by_waves(const Rows &in, int k)
 {
-    return k > 32 || in.C > kBestLabels || (in.sc == 1 && in.C >= 256) || (in.C >= 1024 && in.rows <= 4096);
+    return k > 32 || in.C > kBestLabels || (in.sc == 1 && (in.C >= 256 || (in.C >= 64 && in.rows <= 4096))) || (in.C >= 1024 && in.rows <= 4096);
 }
 
 template <typename T>
