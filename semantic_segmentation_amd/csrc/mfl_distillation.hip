@@ -180,6 +180,23 @@ struct RowFlags {
     __device__ float rest(const Teacher &t) const { return t.rest ? r : -INFINITY; }
 };
 
+// The used ones of KB scores as one Excess: the largest first, so that its own 1 is never added
+template <int KB> __device__ inline Excess excess_of(const float (&v)[KB], const bool (&used)[KB], float c2)
+{
+    float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int j = 0; j < KB; ++j) m = used[j] ? fmaxf(m, v[j]) : m;
+    const float ref = finite_or_zero(m);
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+        const bool first = used[j] && v[j] == m && !found;
+        found |= first;
+        s += used[j] && !first ? __builtin_amdgcn_exp2f((v[j] - ref) * c2) : 0.f;
+    }
+    return {m, m == -INFINITY && s == 0.f ? -1.f : s};
+}
+
 // A record as one lane goes over it: f(block) for all of it, from registers where it fits
 template <typename T, int KB, bool ALL> struct LaneRecord {
     const Rows &in;
@@ -204,45 +221,48 @@ template <typename T, int KB, bool ALL> struct LaneRecord {
         Excess sum = kNoExcess;
         bool named = false;
         each([&](const Block<T, KB> &b) {
+            bool used[KB];
 #pragma unroll
-            for (int j = 0; j < KB; ++j) {
-                named |= b.label[j] >= 0;
-                sum = join(sum, b.label[j] >= 0 ? Excess{b.value[j], 0.f} : kNoExcess, t.c2);
-            }
+            for (int j = 0; j < KB; ++j) named |= used[j] = b.label[j] >= 0;
+            const Excess e = excess_of(b.value, used, t.c2);
+            sum = ALL ? e : join(sum, e, t.c2);
         });
         return target_of(t, sum, named, rest);
     }
 };
 
-// Labels c0 .. c0 + CB of a row (what lies behind the last one: -inf)
-template <typename T, int CB> __device__ inline void load_labels(float (&x)[CB], const Rows &in, const T *p, int c0)
+// Labels c0 .. c0 + CB of a row (what lies behind the last one: -inf).  The first SURE of them are there.
+template <int CB, bool LONE> constexpr int kSure = LONE && CB > 8 ? CB - 3 : 1;
+template <int SURE, typename T, int CB> __device__ inline void load_labels(float (&x)[CB], const Rows &in, const T *p, int c0)
 {
     T raw[CB];
     const T *q = p + c0 * in.sc;
 #pragma unroll
     for (int i = 0; i < CB; ++i) {
         raw[i] = *q;
-        q += c0 + i + 1 < in.C ? in.sc : 0;         // (the last one again)
+        q += i + 1 < SURE || c0 + i + 1 < in.C ? in.sc : 0;         // (the last one again)
     }
 #pragma unroll
-    for (int i = 0; i < CB; ++i) x[i] = i == 0 || c0 + i < in.C ? to_float(raw[i]) : -INFINITY;
+    for (int i = 0; i < CB; ++i) x[i] = i < SURE || c0 + i < in.C ? to_float(raw[i]) : -INFINITY;
 }
 
 // Adds a block of labels to the two sums: the record's into top (each once), the others into out
-template <typename T, int CB, int KB, bool ALL>
+template <typename T, int CB, bool LONE, int KB, bool ALL>
 __device__ inline void add_labels(const LaneRecord<T, KB, ALL> &record, const float (&x)[CB], int c0, float c2, LogSum &out, Excess &top)
 {
     static_assert(CB <= 32, "one word of marks");
     uint32_t marks = 0;
     record.each([&](const Block<T, KB> &b) {
+        bool used[KB];
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
             const int i = b.label[j] - c0;
-            const bool here = b.label[j] >= 0 && (unsigned)i < (unsigned)CB;
-            const uint32_t bit = here ? 1u << i : 0u;
-            top = join(top, here && !(marks & bit) ? Excess{b.x[j], 0.f} : kNoExcess, c2);
+            const uint32_t bit = b.label[j] >= 0 && (LONE || (unsigned)i < (unsigned)CB) ? 1u << (i & 31) : 0u;
+            used[j] = (bit & ~marks) != 0;
             marks |= bit;
         }
+        const Excess e = excess_of(b.x, used, c2);
+        top = LONE && ALL ? e : join(top, e, c2);
     });
     float m = out.m, y[CB];
 #pragma unroll
@@ -266,19 +286,20 @@ forward_lanes_kernel(Rows in, Teacher t, float *__restrict__ loss, float *__rest
     if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
+    constexpr int SURE = kSure<CB, LONE>;
     // (everything is asked for before anything is looked at)
     LaneRecord<T, KB, ALL> record(in, t, p, (size_t)n * t.k * in.S + s);
     float x[CB];
-    load_labels(x, in, p, 0);
+    load_labels<SURE>(x, in, p, 0);
     const RowFlags flags(t, r);
     record.fetch();
     LogSum out = {-INFINITY, 0.f};
     Excess top = kNoExcess;
     for (int c0 = 0;;) {
-        add_labels(record, x, c0, t.c2, out, top);
+        add_labels<T, CB, LONE>(record, x, c0, t.c2, out, top);
         c0 += CB;
         if (LONE || c0 >= in.C) break;
-        load_labels(x, in, p, c0);
+        load_labels<SURE>(x, in, p, c0);
     }
     const Target g = record.target(flags.rest(t));
     const Stats a = stats_of(top, out, t);
@@ -301,14 +322,16 @@ backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const
                       long long gn, long long gc, long long gs)
 {
     __shared__ float taken[CB][kLaneThreads];
-    const unsigned r = blockIdx.x * kLaneThreads + threadIdx.x;
+    constexpr int SURE = kSure<CB, LONE>;
+    // (from the last row on: what the forward pass read last is still in the last-level cache)
+    const unsigned r = (gridDim.x - 1 - blockIdx.x) * kLaneThreads + threadIdx.x;
     if (r >= in.rows) return;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
     T *out = grad + (long long)n * gn + (long long)s * gs;
     LaneRecord<T, KB, ALL> record(in, t, p, (size_t)n * t.k * in.S + s);
     float x[CB];
-    load_labels(x, in, p, 0);
+    load_labels<SURE>(x, in, p, 0);
     const RowFlags flags(t, r);
     const float up = grad_loss[r];
     record.fetch();
@@ -316,7 +339,7 @@ backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const
     if constexpr (LONE) {
         LogSum other = {-INFINITY, 0.f};
         Excess top = kNoExcess;
-        add_labels(record, x, 0, t.c2, other, top);
+        add_labels<T, CB, LONE>(record, x, 0, t.c2, other, top);
         a = stats_of(top, other, t);
     } else {
         a = load_stats(stats, in.rows, r);
@@ -330,7 +353,7 @@ backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const
 #pragma unroll
     for (int i = 0; i < CB; ++i) taken[i][threadIdx.x] = -1.f;
     for (int c0 = 0; c0 < (LONE ? 1 : in.C); c0 += CB) {
-        if (c0) load_labels(x, in, p, c0);
+        if (c0) load_labels<SURE>(x, in, p, c0);
         record.each([&](const Block<T, KB> &b) {
 #pragma unroll
             for (int j = 0; j < KB; ++j) {
@@ -343,7 +366,7 @@ backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
             const float share = taken[i][threadIdx.x];
-            if (c0 + i < in.C) from_float(slope(sl, x[i], share, t.c2), w[i * gc]);
+            if (i < SURE || c0 + i < in.C) store_once(slope(sl, x[i], share, t.c2), w + i * gc);
             if (share >= 0.f) taken[i][threadIdx.x] = -1.f;
         }
     }
@@ -538,7 +561,8 @@ backward_rows_kernel(Rows in, Teacher t, int parts, const float *__restrict__ st
     __shared__ float share[MFL_MAX_TOP_LABELS];
     constexpr int V = kVec<T>;
     const int lane = threadIdx.x & 63;
-    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    // (from the last row on: what the forward pass read last is still in the last-level cache)
+    const unsigned q = blockIdx.x / parts, part = blockIdx.x - q * parts, r = in.rows - 1 - q;
     const unsigned n = r / in.S, s = r - n * in.S;
     const T *p = (const T *)in.p + (long long)n * in.sn + (long long)s * in.ss;
     T *out = grad + (long long)n * gn + (long long)s * gs;
@@ -597,7 +621,7 @@ backward_rows_kernel(Rows in, Teacher t, int parts, const float *__restrict__ st
         for (; c + (U - 1) * kRowThreads * V + V <= c1; c += U * kRowThreads * V) {
             float x[U][V];
 #pragma unroll
-            for (int u = 0; u < U; ++u) load_vec(p + c + u * kRowThreads * V, x[u]);
+            for (int u = 0; u < U; ++u) unpack<T>(load_words_once(p + c + u * kRowThreads * V), x[u]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 turn(x[u], c + u * kRowThreads * V);
@@ -629,17 +653,25 @@ size_t mark_bytes(int C, int parts)
     const int size = part_labels(C, parts);
     return (size_t)(size < kSegment ? size : kSegment) / 8;
 }
-constexpr unsigned kEnough = 2048;      // workgroups that fill the card: 256 CUs, eight each
+constexpr unsigned kEnough = 8192;      // workgroups: 32 for each of 256 CUs, so that the last ones end together
 
 // labels and entries a lane takes at a time
 #define MFL_BY_SIZE(C, k, LAUNCH)                                                             \
     do {                                                                                      \
-        if (C <= 8) {                                                                         \
-            if (k <= 4) LAUNCH(8, true, 4, true);                                             \
-            else LAUNCH(8, true, 8, false);                                                   \
-        } else if (C <= kLoneBlock) {                                                         \
-            if (k <= 4) LAUNCH(kLoneBlock, true, 4, true);                                    \
-            else LAUNCH(kLoneBlock, true, 8, false);                                          \
+        if (C <= kLoneBlock) {                                                                \
+            if (k <= 4) {                                                                     \
+                if (C <= 8) LAUNCH(8, true, 4, true);                                         \
+                else if (C <= 12) LAUNCH(12, true, 4, true);                                  \
+                else if (C <= 16) LAUNCH(16, true, 4, true);                                  \
+                else if (C <= 20) LAUNCH(20, true, 4, true);                                  \
+                else LAUNCH(24, true, 4, true);                                               \
+            } else {                                                                          \
+                if (C <= 8) LAUNCH(8, true, 8, false);                                        \
+                else if (C <= 12) LAUNCH(12, true, 8, false);                                 \
+                else if (C <= 16) LAUNCH(16, true, 8, false);                                 \
+                else if (C <= 20) LAUNCH(20, true, 8, false);                                 \
+                else LAUNCH(24, true, 8, false);                                              \
+            }                                                                                 \
         } else {                                                                              \
             if (k <= 4) LAUNCH(32, false, 4, true);                                           \
             else if (k <= 8) LAUNCH(32, false, 8, true);                                      \

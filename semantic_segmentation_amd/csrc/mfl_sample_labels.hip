@@ -127,7 +127,7 @@ template <int CB> __device__ inline void pick(const double (&w)[CB], double run,
     }
 }
 
-// All labels in registers
+// All labels in registers.  The label is the number of running sums up to the target.
 template <typename T, int CB>
 __global__ void __launch_bounds__(kLaneThreads)
 plain_lone_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
@@ -142,14 +142,28 @@ plain_lone_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out 
     const float m = largest_of(x, -INFINITY);
     if (!(fabsf(m) < INFINITY)) return put(out, r, -1, -INFINITY);
     const Weight weight = {m, f.inv_t * kLog2eD};
-    double w[CB], total = 0;
-    weights_of(w, x, weight, f.min_p);
+    double upto[CB], total = 0;
 #pragma unroll
-    for (int i = 0; i < CB; ++i) total += w[i];
-    int label = -1;
-    double got = 0;
-    pick(w, 0.0, draw_of(u) * total, label, got);
-    put(out, r, label, log(got / total));
+    for (int i = 0; i < CB; ++i) {
+        if (i == 0 || i + 4 <= CB || i < in.C) {        // (of the last ones, only those that are there)
+            const double v = weight(x[i]);
+            total += v >= f.min_p ? v : 0.0;
+        }
+        upto[i] = total;
+    }
+    const double target = draw_of(u) * total;
+    int label = 0;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) label += upto[i] <= target;
+    if (label >= in.C) {                // past all of it: the last one that weighs something
+        double before = 0;
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            label = upto[i] > before ? i : label;
+            before = upto[i];
+        }
+    }
+    put(out, r, label, log(weight(to_float(row.p[label * in.sc])) / total));
 }
 
 struct LaneSums {
@@ -1267,6 +1281,7 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
     switch (plan.way) {
     case LONE:
         if (in.C <= 8) MFL_LANES((plain_lone_kernel<T, 8>));
+        else if (in.C <= 16) MFL_LANES((plain_lone_kernel<T, 16>));
         else MFL_LANES((plain_lone_kernel<T, kLoneBlock>));
         break;
     case LANES: MFL_LANES((plain_lanes_kernel<T>)); break;

@@ -39,6 +39,8 @@ typedef uint32_t words4 __attribute__((ext_vector_type(4)));
 typedef words4 words4_at2 __attribute__((aligned(2)));
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 template <typename T> __device__ inline words4 load_words(const T *p) { return *(const words4_at2 *)p; }
+// ... of data that is not read again soon
+template <typename T> __device__ inline words4 load_words_once(const T *p) { return __builtin_nontemporal_load((const words4_at2 *)p); }
 template <typename T> __device__ inline void unpack(words4 w, float (&x)[kVec<T>])
 {
 #pragma unroll
@@ -50,6 +52,7 @@ template <typename T> __device__ inline void unpack(words4 w, float (&x)[kVec<T>
     }
 }
 template <typename T> __device__ inline void load_vec(const T *p, float (&x)[kVec<T>]) { unpack<T>(load_words(p), x); }
+// (streamed past the caches: a gradient of many labels does not stay in them)
 template <typename T> __device__ inline void store_vec(T *p, const float (&x)[kVec<T>])
 {
     words4 w;
@@ -64,7 +67,7 @@ template <typename T> __device__ inline void store_vec(T *p, const float (&x)[kV
             w[i] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | (uint32_t)__builtin_bit_cast(uint16_t, hi) << 16;
         }
     }
-    *(words4_at2 *)p = w;
+    __builtin_nontemporal_store(w, (words4_at2 *)p);
 }
 
 // Values of a tensor whose type is known at run time only (the teacher's side): all bits first, so that the loads of a
@@ -85,6 +88,15 @@ template <int N, typename At> __device__ inline void load_any(float (&v)[N], con
         const float b = __builtin_bit_cast(float, dtype == MFL_BF16 ? raw[j] << 16 : raw[j]);
         v[j] = dtype == MFL_F16 ? h : b;
     }
+}
+
+// one score, streamed past the caches
+template <typename T> __device__ inline void store_once(float v, T *p)
+{
+    T o;
+    from_float(v, o);
+    if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, o), (uint32_t *)p);
+    else __builtin_nontemporal_store(__builtin_bit_cast(uint16_t, o), (uint16_t *)p);
 }
 
 // Order of scores as signed integers: -inf < ... < -0 = +0 < ... < +inf < NaN
