@@ -684,6 +684,7 @@ int run_forward(const Rows &in, const Teacher &t, float *loss, float *stats, voi
 {
     if (by_rows(in)) {
         const int parts = parts_of(in, kEnough);
+        if (!launchable((unsigned long long)in.rows * parts, kRowThreads)) return MFL_ERR_TOO_LARGE;
         hipLaunchKernelGGL(outside_parts_kernel<T>, dim3(in.rows * parts), dim3(kRowThreads), mark_bytes(in.C, parts), st, in, t, parts,
                            (LogSum *)workspace);
         const unsigned per = kRowThreads / 64;
@@ -704,6 +705,7 @@ int run_backward(const Rows &in, const Teacher &t, const float *stats, const flo
 {
     if (by_rows(in) && out.sc == 1) {
         const int parts = parts_of(in, kEnough);
+        if (!launchable((unsigned long long)in.rows * parts, kRowThreads)) return MFL_ERR_TOO_LARGE;
         hipLaunchKernelGGL(backward_rows_kernel<T>, dim3(in.rows * parts), dim3(kRowThreads), mark_bytes(in.C, parts), st, in, t, parts,
                            stats, grad_loss, (T *)grad, out.sn, out.ss);
         return (int)hipGetLastError();

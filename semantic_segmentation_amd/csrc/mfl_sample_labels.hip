@@ -1276,6 +1276,12 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
 {
     const Plan plan = plan_of(in, set);
     const int k = plan.k;
+    const unsigned threads_a_row = plan.way == PLAIN  ? kPlainThreads * plain_parts(in.rows, in.C)
+                                   : plan.way < PLAIN ? 1
+                                   : plan.way == WAVES && !plan.two && row_per_wave(in.rows, in.C) ? 64
+                                   : plan.way == WAVES && !plan.two ? kWaveTopThreads * top_parts(in.rows, in.C)
+                                                                    : 1024;
+    if (!launchable(in.rows, threads_a_row)) return MFL_ERR_TOO_LARGE;
     const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
 #define MFL_LANES(...) hipLaunchKernelGGL(__VA_ARGS__, grid, block, 0, st, in, set, uniform, out)
     switch (plan.way) {

@@ -267,6 +267,9 @@ struct Weight {
     }
 };
 
+// Host: a launch's threads are counted in 32 bits
+inline bool launchable(unsigned long long blocks, unsigned threads) { return blocks * threads < (1ull << 32); }
+
 // Host: the arguments every call shares.  0 or an error code; fills the view.
 inline int make_rows(Rows &r, const void *p, int dtype, int N, int C, int S, long long sn, long long sc, long long ss)
 {

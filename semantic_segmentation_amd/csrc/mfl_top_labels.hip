@@ -151,6 +151,8 @@ int run(const Rows &in, double temperature, int k, void *values, int *labels, fl
 {
     const float c2 = (float)(kLog2eD / temperature), inv_t = (float)(1.0 / temperature);
     if (by_waves(in, k)) {
+        if (!launchable((unsigned long long)in.rows * (row_per_wave(in.rows, in.C) ? 1 : top_parts(in.rows, in.C)), kWaveTopThreads))
+            return MFL_ERR_TOO_LARGE;
         if (row_per_wave(in.rows, in.C)) {
             const unsigned per = kWaveTopThreads / 64;
             hipLaunchKernelGGL(top_waves_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kWaveTopThreads), 0, st, in, c2, inv_t, k,

@@ -79,7 +79,7 @@ def check_top(S, x, k, t):
 
 TOP_SHAPES = [((1, 1), 1), ((3, 2), 2), ((2, 5, 3, 7), 3), ((1, 21, 9, 31), 4), ((2, 33, 4, 65), 8), ((1, 150, 5, 13), 16),
               ((2, 40, 3), 32), ((1, 40, 7), 40), ((3, 127), 127), ((2, 129), 128), ((5, 511), 8), ((3, 512), 1), ((4, 513), 65),
-              ((2, 4097), 128), ((1, 70001), 50), ((70, 1030), 7), ((300, 600), 20)]
+              ((2, 4097), 128), ((1, 70001), 50), ((70, 1030), 7), ((300, 600), 20), ((2, 1100, 3), 20), ((1, 20000), 128), ((5000, 70), 33)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -153,7 +153,7 @@ def check_distill(S, x, values, labels, rest, t, valid=None, weight=None):
 
 DISTILL_SHAPES = [((1, 1), 1), ((3, 2), 1), ((2, 5, 3, 7), 5), ((1, 21, 9, 31), 4), ((2, 33, 4, 65), 8), ((1, 150, 5, 13), 16),
                   ((2, 300, 9), 40), ((3, 127), 127), ((5, 511), 8), ((3, 512), 128), ((4, 513), 3), ((2, 4097), 64), ((1, 70001), 50),
-                  ((70, 1030), 7)]
+                  ((70, 1030), 7), ((2, 1100, 3), 20), ((1, 12, 7, 9), 2), ((1, 17, 7, 9), 9), ((1, 64, 130, 127), 20)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -304,7 +304,22 @@ def test_sample_labels(shape, dtype, S):
         check_sample(S, y, u, min_p=0.01)
 
 
-@pytest.mark.parametrize("shape", [(9, 40), (9, 30, 2, 3), (9, 1500)])
+@pytest.mark.parametrize("scale", [0.1, 2.0])
+@pytest.mark.parametrize("shape,dtype", [((1, 70, 50, 60), torch.float32), ((2, 150, 33, 40), torch.bfloat16), ((1, 30, 60, 50), torch.float16),
+                                         ((2, 1500, 3), torch.float32)])
+def test_sample_labels_of_maps_with_flat_and_peaked_rows(shape, dtype, scale, S):
+    """Enough pixels for one lane each; flat rows keep far more labels than a lane's list holds."""
+    x = scores_of(shape, dtype, 70, scale)
+    u = torch.rand((shape[0],) + tuple(shape[2:]), generator=gen(71), device="cuda")
+    for kw in (dict(top_p=0.9), dict(top_p=0.55, min_p=0.02), dict(top_k=45), dict(top_k=60, top_p=0.7), dict(top_k=20, top_p=0.8)):
+        check_sample(S, x, u, **kw)
+    f = lambda *v: torch.tensor(v[:shape[0]], dtype=torch.float32, device="cuda")
+    check_sample(S, x, u, temperature=f(0.7, 1.5), top_p=f(0.8, 0.95), min_p=f(0.0, 0.01),
+                 top_k=torch.tensor([0, 50][:shape[0]], dtype=torch.int32, device="cuda"))
+    check_sample(S, x, u, temperature=f(1.3, 0.0))
+
+
+@pytest.mark.parametrize("shape", [(9, 40), (9, 30, 2, 3), (9, 1500), (9, 9000)])
 def test_sample_labels_with_settings_of_every_row(shape, S):
     x = scores_of(shape, torch.float32, 73, 2.0)
     u = torch.rand((shape[0],) + tuple(shape[2:]), generator=gen(74), device="cuda")
@@ -499,7 +514,8 @@ def test_teacher_to_student_on_the_mean_field_modules(S):
     rows = 4.0 * (a.exp() * (a - q)).sum(1) * valid
     want = (rows.flatten(1).sum(1) / valid.flatten(1).sum(1)).mean()
     want.backward()
-    assert abs(float(loss) - float(want)) <= 1e-5 * abs(float(want))
+    loss, want = float(loss.detach()), float(want.detach())
+    assert abs(loss - want) <= 1e-5 * abs(want)
     for name, p in student.named_parameters():
         scale = float(p.grad.abs().max())
         assert float((got[name] - p.grad).abs().max()) <= 1e-4 * scale, name

@@ -65,6 +65,29 @@ def test_sample_labels_refuses(L):
         assert call(**kw) == -1
 
 
+def test_launches_past_32_bits_of_threads_are_refused(L):
+    """2^25 rows of 300 labels would take one wave or workgroup each: more threads than a launch counts."""
+    v = view(N=1 << 25, C=300, S=1, strides=(300, 1, 1))
+    assert top(L, v) == -3
+    assert L.mfl_distillation_forward(*view(N=1 << 25, C=600, S=1, strides=(600, 1, 1)), one, F32, one, None, None, 2, 1.0, one, one, one,
+                                      1 << 40, None) == -3
+    assert L.mfl_sample_labels(*v, one, 1.0, None, 0, None, 0.5, None, 0.0, None, one, 8, None, None, 0, None) == -3
+
+
+def test_workspaces(L):
+    """Small calls take none; a missing or short one is refused before any launch."""
+    assert L.mfl_top_labels_workspace_bytes(8, 21, 4096, F32, 4) == 0
+    n = L.mfl_top_labels_workspace_bytes(1, 128000, 1, F32, 50)
+    assert n > 0
+    v = view(N=1, C=128000, S=1, strides=(128000, 1, 1))
+    assert L.mfl_top_labels(*v, 1.0, 50, one, one, one, None, 0, None) == -2
+    assert L.mfl_top_labels(*v, 1.0, 50, one, one, one, one, n - 1, None) == -2
+    m = L.mfl_distillation_workspace_bytes(1, 128000, 1, F32, 50)
+    assert m > 0 and L.mfl_distillation_forward(*v, one, F32, one, None, None, 2, 1.0, one, one, one, m - 1, None) == -2
+    q = L.mfl_sample_labels_workspace_bytes(1, 128000, 1, F32)
+    assert q > 0 and L.mfl_sample_labels(*v, one, 1.0, None, 0, None, 1.0, None, 0.0, None, one, 8, None, None, 0, None) == -2
+
+
 def test_wrappers_refuse_host_tensors_and_wrong_types():
     import semantic_segmentation_amd as S
     x, u = torch.zeros(2, 5, 4), torch.zeros(2, 4)
