@@ -184,6 +184,8 @@ def _score_rows(t: torch.Tensor, name: str = "scores"):
     if total == 0:
         raise RuntimeError(f"{name} is empty: {tuple(shape)}")
     N, C = shape[0], shape[1]
+    if total // C > 0x7fffffff or C > 1 << 30:             # (they travel as 32-bit numbers)
+        raise ValueError(f"{name} {tuple(shape)}: at most 2^31 - 1 rows of at most 2^30 labels")
     if t.is_contiguous():
         S = total // (N * C)
         return t, (t.data_ptr(), code, N, C, S, C * S, S, 1)
@@ -310,6 +312,10 @@ def sample_labels(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         if torch.is_tensor(x):
             keep.append(_beside(scores, x, name, kinds, (N,)))
             settings += [0, keep[-1].data_ptr()]
+        elif kinds is _I32:
+            if x < 0:
+                raise ValueError(f"top_k must not be negative, got {x}")
+            settings += [min(int(x), 0x7fffffff), None]
         else:
             settings += [x, None]
     labels = torch.empty(rows, dtype=dtype, device=scores.device)
