@@ -648,8 +648,69 @@ template <typename V, int NT> __device__ inline V block_front(V v, V *part, V &a
     return before + (lane ? ahead : V(0));
 }
 
-template <typename T, int NT> struct BlockRow {
-    static constexpr int kBins = 4 * NT, V = kVec<T>, step = 64 * V, waves = NT / 64;
+// What the listed keys above one hold.  The list ends in zeros up to a multiple of eight, so that eight are on their way at once.
+MFL_INLINE unsigned long long held_above(const unsigned long long *keys, const unsigned long long *masses, int n, uint64_t key)
+{
+    unsigned long long above = 0;
+    for (int j = 0; j < n; j += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) above += keys[j + i] > key ? masses[j + i] : 0;
+    }
+    return above;
+}
+
+// Bins of (largest - score) / T and fixed-point masses of a row
+template <int BINS> struct Bins {
+    static constexpr int kBins = BINS;
+    float m, scale;
+    Weight weight;
+    int bits;                   // of the masses
+
+    MFL_INLINE explicit Bins(int C)
+    {
+        const int wide = 32 - __builtin_clz(C);     // C < 2^wide
+        bits = min(51, 62 - wide);
+    }
+    MFL_INLINE void set(float largest, const Filter &f)
+    {
+        m = largest;
+        scale = (float)fmin(f.inv_t * (BINS / kUnits), 1e30);
+        weight = {m, f.inv_t * kLog2eD};
+    }
+    MFL_INLINE int bin_of(float x) const { return min((int)((m - x) * scale), BINS - 1); }
+    MFL_INLINE uint64_t mass(float x) const
+    {
+        // 2^52 + an integer below 2^52: the low bits of the sum are that integer
+        const double v = __builtin_ldexp(weight(x), bits) + 4503599627370496.0;
+        return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
+    }
+    // The lowest score of bins 0 .. b (they grow as the score falls); b = -1: none
+    MFL_INLINE float lowest_of(int b) const
+    {
+        if (b < 0) return INFINITY;
+        // hi is in, lo is not; 64 places between them at a time, one a lane
+        long long lo = score_key(-INFINITY), hi = score_key(m);
+        if (bin_of(-INFINITY) <= b) return -INFINITY;
+#pragma unroll 1
+        while (hi - lo > 1) {
+            const long long step = (hi - lo + 63) >> 6, at = min(lo + ((threadIdx.x & 63) + 1) * step, hi);
+            const int in = __ffsll((unsigned long long)__ballot(bin_of(key_score((int)at)) <= b)) - 1;
+            hi = min(lo + (in + 1) * step, hi);
+            lo += in * step;
+        }
+        return key_score((int)hi);
+    }
+};
+
+template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
+    using Bins<4 * NT>::kBins;
+    using Bins<4 * NT>::m;
+    using Bins<4 * NT>::weight;
+    using Bins<4 * NT>::bits;
+    using Bins<4 * NT>::bin_of;
+    using Bins<4 * NT>::mass;
+    using Bins<4 * NT>::lowest_of;
+    static constexpr int V = kVec<T>, step = 64 * V, waves = NT / 64;
     struct Shared {
         uint32_t counts[kBins];
         unsigned long long masses[kBins];
@@ -666,31 +727,13 @@ template <typename T, int NT> struct BlockRow {
     const T *p;
     long long sc;
     int C;
-    float m, scale;
-    Weight weight;
-    int bits;                   // of the fixed-point masses
     int tiles, per, count_runs; // 64 lanes' vectors of labels, tiles a run, runs
 
-    MFL_INLINE BlockRow(Shared &sh, const T *p, long long sc, int C) : sh(sh), p(p), sc(sc), C(C)
+    MFL_INLINE BlockRow(Shared &sh, const T *p, long long sc, int C) : Bins<4 * NT>(C), sh(sh), p(p), sc(sc), C(C)
     {
-        const int wide = 32 - __builtin_clz(C);     // C < 2^wide
-        bits = min(51, 62 - wide);
         tiles = (C + step - 1) / step;
         per = (tiles + kRuns - 1) / kRuns;
         count_runs = (tiles + per - 1) / per;
-    }
-    MFL_INLINE void set(const Filter &f)
-    {
-        scale = (float)fmin(f.inv_t * (kBins / kUnits), 1e30);
-        weight = {m, f.inv_t * kLog2eD};
-    }
-
-    MFL_INLINE int bin_of(float x) const { return min((int)((m - x) * scale), kBins - 1); }
-    MFL_INLINE uint64_t mass(float x) const
-    {
-        // 2^52 + an integer below 2^52: the low bits of the sum are that integer
-        const double v = __builtin_ldexp(weight(x), bits) + 4503599627370496.0;
-        return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
     }
     // f(score, label) over the row
     template <typename F> MFL_INLINE void each(F f) const
@@ -722,7 +765,7 @@ template <typename T, int NT> struct BlockRow {
         }
     }
 
-    MFL_INLINE void largest()
+    MFL_INLINE float largest()
     {
         float v = -INFINITY;
         each([&](float x, int) __attribute__((always_inline)) { v = max_or_nan(v, x); });
@@ -731,7 +774,7 @@ template <typename T, int NT> struct BlockRow {
         if ((threadIdx.x & 63) == 0) sh.fpart[threadIdx.x >> 6] = v;
         __syncthreads();
         for (int w = 0; w < NT / 64; ++w) v = max_or_nan(v, sh.fpart[w]);
-        m = v;
+        return v;
     }
 
     // A lane's vector of a tile (behind the last label: -inf)
@@ -774,21 +817,6 @@ template <typename T, int NT> struct BlockRow {
             for (int u = 0; u < U; ++u)
                 if (lane == 0 && e + u * waves < count_runs) sh.runs[e + u * waves] = sum[u];
         }
-    }
-
-    // The lowest score of bins 0 .. b (they grow as the score falls); b = -1: none
-    MFL_INLINE float lowest_of(int b) const
-    {
-        if (b < 0) return INFINITY;
-        int lo = score_key(-INFINITY), hi = score_key(m);       // hi is in, lo is not
-        if (bin_of(-INFINITY) <= b) return -INFINITY;
-#pragma unroll 1
-        while (hi - (long long)lo > 1) {
-            const int mid = (int)(((long long)lo + hi) >> 1);
-            if (bin_of(key_score(mid)) <= b) hi = mid;
-            else lo = mid;
-        }
-        return key_score(hi);
     }
 
     // sh.runs = the runs' weights of at least min_p of scores from `sure` on, and, unless LIST, of scores from `open` on
@@ -883,12 +911,14 @@ template <typename T, int NT> struct BlockRow {
             sweep<true>(sure, open, cut, f.min_p);
             const int n = sh.listed;
             if (n <= kBinList) {
-                for (int i = threadIdx.x; i < n; i += NT) sh.key_mass[i] = count ? 1 : mass(rank_score(sh.key[i]));
+                for (int i = threadIdx.x; i < (n + 7) / 8 * 8; i += NT) {
+                    if (i >= n) sh.key[i] = 0;
+                    sh.key_mass[i] = i >= n ? 0 : count ? 1 : mass(rank_score(sh.key[i]));
+                }
                 __syncthreads();
                 for (int i = threadIdx.x; i < n; i += NT) {
                     const uint64_t key = sh.key[i];
-                    unsigned long long above = 0;
-                    for (int j = 0; j < n; ++j) above += sh.key[j] > key ? sh.key_mass[j] : 0;
+                    const unsigned long long above = held_above(sh.key, sh.key_mass, n, key);
                     // (a goal of next to nothing still keeps the first label)
                     if (front + above == 0 || (double)(front + above) < goal) {
                         atomicMin(&sh.low_key, key);
@@ -1037,12 +1067,12 @@ sample_blocks_kernel(Rows in, Settings set, int done, const float *__restrict__ 
     const Filter f = filter_of(set, at.n, in.C);
     if (f.top_k <= done) return;            // (a list had it)
     BlockRow<T, NT> row(sh, at.p, in.sc, in.C);
-    row.largest();
-    if (!(fabsf(row.m) < INFINITY)) {
+    const float m = row.largest();
+    if (!(fabsf(m) < INFINITY)) {
         if (threadIdx.x == 0) put(out, r, -1, -INFINITY);
         return;
     }
-    row.set(f);
+    row.set(m, f);
     const uint64_t cut = row.cut_of(f);
     row.draw(cut, f.min_p, uniform[r], r, out);
 }
@@ -1136,13 +1166,89 @@ plain_parts_kernel(Rows in, Settings set, int parts, int size, Part *__restrict_
     }
 }
 
+// Of n entries, the first whose running sum from front0 on exceeds the target, or the last that holds something; *before: the
+// sum in front of it.  Unless given, all = the sum of the entries and target = its share u.
+template <typename F>
+__device__ inline int find_entry(int n, F value, double front0, float u, double &target, double &all, bool given, double *dpart, unsigned *first,
+                                 unsigned *last, double *before)
+{
+    const int each = (n + kPlainThreads - 1) / kPlainThreads, from = min(n, (int)threadIdx.x * each), to = min(n, from + each);
+    double mine = 0;
+    int holds = -1;
+    for (int i = from; i < to; ++i) {
+        const double v = value(i);
+        mine += v;
+        if (v > 0) holds = i;
+    }
+    double sum, front = front0 + block_front<double, kPlainThreads>(mine, dpart, sum);
+    if (!given) {
+        all = sum;
+        target = draw_of(u) * all;
+    }
+    if (threadIdx.x == 0) *first = ~0u, *last = 0;
+    __syncthreads();
+    if (holds >= 0) atomicMax(last, (unsigned)holds);
+    if (mine > 0 && front + mine > target) {
+        double run = front;
+        for (int i = from; i < to; ++i) {
+            run += value(i);
+            if (run > target) {
+                atomicMin(first, (unsigned)i);
+                break;
+            }
+        }
+    }
+    __syncthreads();
+    const int at = *first != ~0u ? (int)*first : (int)*last;
+    if (at >= from && at < to) {
+        for (int i = from; i < at; ++i) front += value(i);
+        *before = front;
+    }
+    __syncthreads();
+    return at;
+}
+// The label within the part that the draw falls into; kept(score, label) is what a label weighs
+template <typename T, typename F>
+__device__ inline void pick_in_part(const T *p, long long sc, int begin, int end, F kept, double front, double target, double total, double *sums,
+                                    double *dpart, unsigned *first, unsigned *last, double *before, unsigned r, const Out &out)
+{
+    constexpr int V = kVec<T>, U = kPlainVecs<T>;
+    float x[U][V];
+    load_part(x, p, sc, begin, end);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = begin + (u * kPlainThreads + (int)threadIdx.x) * V;
+        double s = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += kept(x[u][i], c + i);
+        sums[u * kPlainThreads + threadIdx.x] = s;
+    }
+    __syncthreads();
+    const int vec = find_entry(U * kPlainThreads, [&](int i) { return sums[i]; }, front, 0.f, target, total, true, dpart, first, last, before);
+    // (its scores are still in the registers of the thread that summed it)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (vec != u * kPlainThreads + (int)threadIdx.x) continue;
+        double run = *before, got = 0;
+        int label = -1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double w = kept(x[u][i], begin + vec * V + i);
+            const bool open = w > 0 && !(label >= 0 && run > target);
+            run += open ? w : 0.0;
+            label = open ? begin + vec * V + i : label;
+            got = open ? w : got;
+        }
+        put(out, r, label, log(got / total));
+    }
+}
+
 template <typename T, bool AGAIN>
 __global__ void __launch_bounds__(kPlainThreads)
 plain_pick_kernel(Rows in, Settings set, int parts, int size, const Part *__restrict__ ws, const float *__restrict__ uniform, Out out)
 {
-    constexpr int V = kVec<T>, U = kPlainVecs<T>;
     __shared__ float fpart[kPlainThreads / 64];
-    __shared__ double dpart[kPlainThreads / 64], sums[U * kPlainThreads], before;
+    __shared__ double dpart[kPlainThreads / 64], sums[kPlainVecs<T> * kPlainThreads], before;
     __shared__ unsigned first, last;
     const unsigned r = blockIdx.x;
     const RowOf<T> row(in, r);
@@ -1154,76 +1260,228 @@ plain_pick_kernel(Rows in, Settings set, int parts, int size, const Part *__rest
         return;
     }
     const Weight weight = {m, f.inv_t * kLog2eD};
-    auto scaled = [&](int i) { return AGAIN ? ws[i].sum : ws[i].sum * weight(ws[i].top); };
-    // the first of n entries whose running sum exceeds the target, or the last that holds something; what lies in front
-    auto find = [&](int n, auto value, double front0, double &target, double &all, bool given) {
-        const int each = (n + kPlainThreads - 1) / kPlainThreads, from = min(n, (int)threadIdx.x * each), to = min(n, from + each);
-        double mine = 0;
-        int holds = -1;
-        for (int i = from; i < to; ++i) {
-            const double v = value(i);
-            mine += v;
-            if (v > 0) holds = i;
-        }
-        double sum, front = front0 + block_front<double, kPlainThreads>(mine, dpart, sum);
-        if (!given) {
-            all = sum;
-            target = draw_of(uniform[r]) * all;
-        }
-        if (threadIdx.x == 0) first = ~0u, last = 0;
-        __syncthreads();
-        if (holds >= 0) atomicMax(&last, (unsigned)holds);
-        if (mine > 0 && front + mine > target) {
-            double run = front;
-            for (int i = from; i < to; ++i) {
-                run += value(i);
-                if (run > target) {
-                    atomicMin(&first, (unsigned)i);
-                    break;
-                }
-            }
-        }
-        __syncthreads();
-        const int at = first != ~0u ? (int)first : (int)last;
-        if (at >= from && at < to) {
-            for (int i = from; i < at; ++i) front += value(i);
-            before = front;
-        }
-        __syncthreads();
-        return at;
-    };
     double target = 0, total = 0;
-    const int part = find(parts, scaled, 0.0, target, total, false);
+    const int part = find_entry(parts, [&](int i) { return AGAIN ? ws[i].sum : ws[i].sum * weight(ws[i].top); }, 0.0, uniform[r], target, total, false,
+                                dpart, &first, &last, &before);
     const double front = before;
     __syncthreads();
-    const int begin = part * size, end = min(in.C, begin + size);
-    float x[U][V];
-    load_part(x, row.p, in.sc, begin, end);
-    auto kept = [&](float v) {
+    auto kept = [&](float v, int) {
         const double w = weight(v);
         return w >= f.min_p ? w : 0.0;
     };
+    pick_in_part<T>(row.p, in.sc, part * size, min(in.C, part * size + size), kept, front, target, total, sums, dpart, &first, &last, &before, r, out);
+}
+
+// ---- few rows of many labels that top_p cuts: the workgroup's steps, spread over the card
+//
+//   1  the parts' largest scores               2  the histogram: a part's in LDS, then added to the row's (integers)
+//   3  every workgroup finds the row's bin for itself; its part's sure weights summed, the bin's labels listed
+//   4  one workgroup per row: the cut within the list, the part, the label.  (A list that overflowed, or a top_k of the row's
+//      own: all of the workgroup's steps.)
+
+constexpr int kSplitBins = 4096;
+constexpr int kSplitParts = 512;
+constexpr unsigned kSplitRows = 128;
+struct SplitRow {
+    unsigned long long masses[kSplitBins], keys[kBinList];
+    unsigned long long front;
+    double goal;
+    unsigned listed;
+};
+struct SplitSpace {
+    SplitRow *rows;
+    Part *parts;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kPlainThreads)
+split_largest_kernel(Rows in, int parts, int size, SplitSpace ws)
+{
+    __shared__ float fpart[kPlainThreads / 64];
+    constexpr int V = kVec<T>, U = kPlainVecs<T>;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const RowOf<T> row(in, r);
+    float x[U][V], m = -INFINITY;
+    load_part(x, row.p, in.sc, part * size, min(in.C, (int)part * size + size));
+    for (int b = part * kPlainThreads + threadIdx.x; b < kSplitBins; b += parts * kPlainThreads) ws.rows[r].masses[b] = 0;
+    if (part == 0 && threadIdx.x == 0) ws.rows[r].listed = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = largest_of(x[u], m);
+    m = block_largest(m, fpart);
+    if (threadIdx.x == 0) ws.parts[blockIdx.x].top = m;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPlainThreads)
+split_histogram_kernel(Rows in, Settings set, int parts, int size, SplitSpace ws)
+{
+    __shared__ unsigned long long masses[kSplitBins];
+    __shared__ float fpart[kPlainThreads / 64];
+    constexpr int V = kVec<T>, U = kPlainVecs<T>;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const RowOf<T> row(in, r);
+    const Filter f = filter_of(set, row.n, in.C);
+    if (f.top_k < in.C || f.top_p >= 1) return;
+    const int begin = part * size, end = min(in.C, begin + size);
+    float x[U][V];
+    load_part(x, row.p, in.sc, begin, end);
+    const float m = largest_of_parts(ws.parts + (size_t)r * parts, parts, fpart);
+    if (!(fabsf(m) < INFINITY)) return;
+    Bins<kSplitBins> bins(in.C);
+    bins.set(m, f);
+    for (int b = threadIdx.x; b < kSplitBins; b += kPlainThreads) masses[b] = 0;
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        double s = 0;
+        const int c = begin + (u * kPlainThreads + (int)threadIdx.x) * V;
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += kept(x[u][i]);
-        sums[u * kPlainThreads + threadIdx.x] = s;
+        for (int i = 0; i < V; ++i) {
+            const uint64_t v = c + i < end ? bins.mass(x[u][i]) : 0;
+            if (v) atomicAdd(&masses[bins.bin_of(x[u][i])], (unsigned long long)v);
+        }
     }
     __syncthreads();
-    const int vec = find(U * kPlainThreads, [&](int i) { return sums[i]; }, front, target, total, true);
-    if (threadIdx.x) return;
-    double run = before, got = 0;
-    int label = -1;
-    for (int c = begin + vec * V; c < min(end, begin + (vec + 1) * V); ++c) {
-        const double w = kept(to_float(row.p[c * in.sc]));
-        if (w == 0) continue;
-        run += w;
-        label = c;
-        got = w;
-        if (run > target) break;
+    for (int b = threadIdx.x; b < kSplitBins; b += kPlainThreads)
+        if (masses[b]) atomicAdd(&ws.rows[r].masses[b], masses[b]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPlainThreads)
+split_sweep_kernel(Rows in, Settings set, int parts, int size, SplitSpace ws)
+{
+    __shared__ float fpart[kPlainThreads / 64];
+    __shared__ double dpart[kPlainThreads / 64];
+    __shared__ unsigned long long upart[kPlainThreads / 64], bin_front;
+    __shared__ int bin;
+    constexpr int V = kVec<T>, U = kPlainVecs<T>, each_bins = kSplitBins / kPlainThreads;
+    const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const RowOf<T> row(in, r);
+    const Filter f = filter_of(set, row.n, in.C);
+    if (f.top_k < in.C) return;
+    const int begin = part * size, end = min(in.C, begin + size);
+    float x[U][V];
+    load_part(x, row.p, in.sc, begin, end);
+    SplitRow &state = ws.rows[r];
+    const float m = largest_of_parts(ws.parts + (size_t)r * parts, parts, fpart);
+    if (!(fabsf(m) < INFINITY)) return;
+    Bins<kSplitBins> bins(in.C);
+    bins.set(m, f);
+    float sure = -INFINITY, open = -INFINITY;
+    if (f.top_p < 1) {
+        unsigned long long masses[each_bins], mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < each_bins; ++i) mine += masses[i] = state.masses[threadIdx.x * each_bins + i];
+        unsigned long long front = block_front<unsigned long long, kPlainThreads>(mine, upart, all);
+        const double goal = f.top_p * (double)all;
+        if (threadIdx.x == 0) bin = 0, bin_front = 0;
+        __syncthreads();
+        if ((double)front < goal && (double)(front + mine) >= goal) {
+            int at = -1;
+            unsigned long long before = 0;
+#pragma unroll
+            for (int i = 0; i < each_bins; ++i) {
+                if (at < 0 && (double)(front + masses[i]) >= goal) at = i, before = front;
+                front += masses[i];
+            }
+            bin = threadIdx.x * each_bins + at;
+            bin_front = before;
+        }
+        __syncthreads();
+        sure = bins.lowest_of(bin - 1);
+        open = bins.lowest_of(bin);
+        if (part == 0 && threadIdx.x == 0) state.front = bin_front, state.goal = goal;
     }
-    put(out, r, label, log(got / total));
+    double sum = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = begin + (u * kPlainThreads + (int)threadIdx.x) * V;
+        uint32_t todo = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) todo |= x[u][i] >= open && c + i < end ? 1u << i : 0u;
+#pragma unroll 1
+        while (__any(todo != 0)) {
+            const int i = __ffs(todo) - 1;
+            float v = x[u][0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) v = i == j ? x[u][j] : v;
+            const bool keep = todo != 0 && v >= sure;
+            if (todo != 0 && !keep) {
+                const unsigned at = atomicAdd(&state.listed, 1u);
+                if (at < (unsigned)kBinList) state.keys[at] = rank_key(score_key(v), c + i);
+            }
+            todo &= todo - 1;
+            const double w = bins.weight(v);
+            sum += keep && w >= f.min_p ? w : 0.0;
+        }
+    }
+    sum = block_sum<double, kPlainThreads>(sum, dpart);
+    if (threadIdx.x == 0) ws.parts[blockIdx.x].sum = sum;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPlainThreads)
+split_pick_kernel(Rows in, Settings set, int done, int parts, int size, SplitSpace ws, const float *__restrict__ uniform, Out out)
+{
+    constexpr int U = kPlainVecs<T>, NT = kPlainThreads;
+    __shared__ typename BlockRow<T, NT>::Shared sh;
+    __shared__ unsigned long long more[kSplitParts];
+    __shared__ double sums[U * NT], before;
+    __shared__ unsigned first, last;
+    const unsigned r = blockIdx.x;
+    const RowOf<T> at(in, r);
+    const Filter f = filter_of(set, at.n, in.C);
+    if (f.top_k <= done) return;            // (a list had it)
+    const Part *part_of = ws.parts + (size_t)r * parts;
+    const SplitRow &state = ws.rows[r];
+    const float m = largest_of_parts(part_of, parts, sh.fpart);
+    if (!(fabsf(m) < INFINITY)) {
+        if (threadIdx.x == 0) put(out, r, -1, -INFINITY);
+        return;
+    }
+    BlockRow<T, NT> row(sh, at.p, in.sc, in.C);
+    row.set(m, f);
+    const bool ranked = f.top_p < 1;
+    const unsigned n = f.top_k < in.C ? ~0u : ranked ? state.listed : 0;
+    if (n > (unsigned)kBinList) {
+        const uint64_t cut = row.cut_of(f);
+        row.draw(cut, f.min_p, uniform[r], r, out);
+        return;
+    }
+    // the cut within the list
+    uint64_t cut = 0;
+    for (int i = threadIdx.x; i < parts; i += NT) more[i] = 0;
+    if (ranked) {
+        if (threadIdx.x == 0) sh.low_key = ~0ull;
+        for (unsigned i = threadIdx.x; i < (n + 7) / 8 * 8; i += NT) {
+            sh.key[i] = i < n ? state.keys[i] : 0;
+            sh.key_mass[i] = i < n ? row.mass(rank_score(sh.key[i])) : 0;
+        }
+        __syncthreads();
+        const unsigned long long front = state.front;
+        const double goal = state.goal;
+        for (unsigned i = threadIdx.x; i < n; i += NT) {
+            const uint64_t key = sh.key[i];
+            const unsigned long long above = held_above(sh.key, sh.key_mass, n, key);
+            if (front + above == 0 || (double)(front + above) < goal) {
+                atomicMin(&sh.low_key, key);
+                if (row.weight(rank_score(key)) >= f.min_p) atomicAdd(&more[rank_label(key) / size], sh.key_mass[i]);
+            }
+        }
+    }
+    __syncthreads();
+    if (ranked) cut = sh.low_key;
+    const float cut_score = cut ? rank_score(cut) : -INFINITY;
+    auto kept = [&](float x, int c) {
+        if (!(x >= cut_score) || rank_key(score_key(x), c) < cut) return 0.0;
+        const double w = row.weight(x);
+        return w >= f.min_p ? w : 0.0;
+    };
+    double target = 0, total = 0;
+    const int part = find_entry(parts, [&](int i) { return part_of[i].sum + __builtin_ldexp((double)more[i], -row.bits); }, 0.0, uniform[r], target, total,
+                                false, sh.dpart, &first, &last, &before);
+    const double front = before;
+    __syncthreads();
+    pick_in_part<T>(at.p, in.sc, part * size, min(in.C, part * size + size), kept, front, target, total, sums, sh.dpart, &first, &last, &before, r, out);
 }
 
 int plain_part_labels(unsigned rows, int C)
@@ -1241,11 +1499,12 @@ int list_length(const Settings &set)
     return set.top_k >= 1 && set.top_k <= MFL_MAX_TOP_LABELS ? set.top_k : 0;
 }
 
-enum Way { LONE, LANES, LIST_LANES, ANY_LANES, PLAIN, WAVES, BLOCKS };
+enum Way { LONE, LANES, LIST_LANES, ANY_LANES, PLAIN, WAVES, SPLIT, BLOCKS };
 struct Plan {
     Way way;
     int k;                      // length of the list, 0: none
-    bool two;                   // WAVES, then BLOCKS for the rows whose own top_k is not that short
+    bool two;                   // WAVES, then SPLIT or BLOCKS for the rows whose own top_k is not that short
+    bool split;
     size_t bytes;
 };
 Plan plan_of(const Rows &in, const Settings &set)
@@ -1260,15 +1519,18 @@ Plan plan_of(const Rows &in, const Settings &set)
     // lanes: short rows, and planes of many rows
     if (!(in.sc == 1 && in.C >= 256) && !(in.C >= 1024 && in.rows <= 4096)) {
         const int list = k ? k : no_k && in.C <= 32 ? in.C : 0;
-        if (plain) return {in.C <= kLoneBlock ? LONE : LANES, 0, false, 0};
-        if (list && list <= 32 && in.C <= kBestLabels) return {LIST_LANES, list, false, 0};
+        if (plain) return {in.C <= kLoneBlock ? LONE : LANES, 0, false, false, 0};
+        if (list && list <= 32 && in.C <= kBestLabels) return {LIST_LANES, list, false, false, 0};
         // (few rows of many labels to rank: a workgroup each)
-        if (in.C <= kBestLabels && (in.rows > 2048 || in.C <= 64)) return {ANY_LANES, 0, false, 0};
+        if (in.C <= kBestLabels && (in.rows > 2048 || in.C <= 64)) return {ANY_LANES, 0, false, false, 0};
     }
-    if (plain && in.C > 4096) return {PLAIN, 0, false, (size_t)in.rows * plain_parts(in.rows, in.C) * sizeof(Part)};
-    if (k) return {WAVES, k, false, keys(k)};
-    if (set.top_k_n && in.C > MFL_MAX_TOP_LABELS) return {WAVES, MFL_MAX_TOP_LABELS, true, keys(MFL_MAX_TOP_LABELS)};
-    return {BLOCKS, 0, false, 0};
+    if (plain && in.C > 4096) return {PLAIN, 0, false, false, (size_t)in.rows * plain_parts(in.rows, in.C) * sizeof(Part)};
+    if (k) return {WAVES, k, false, false, keys(k)};
+    // (a top_k for all rows that is too long for a list is the workgroup's to count)
+    const bool split = in.C > 8192 && in.rows <= kSplitRows && (no_k || set.top_k_n) && plain_parts(in.rows, in.C) <= kSplitParts;
+    const size_t space = split ? (size_t)in.rows * (sizeof(SplitRow) + plain_parts(in.rows, in.C) * sizeof(Part)) : 0;
+    if (set.top_k_n && in.C > MFL_MAX_TOP_LABELS) return {WAVES, MFL_MAX_TOP_LABELS, true, split, space + keys(MFL_MAX_TOP_LABELS)};
+    return {split ? SPLIT : BLOCKS, 0, false, split, space};
 }
 
 template <typename T>
@@ -1315,12 +1577,13 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
         break;
     }
     case WAVES: {
+        const size_t space = plan.split ? (size_t)in.rows * (sizeof(SplitRow) + plain_parts(in.rows, in.C) * sizeof(Part)) : 0;
         if (row_per_wave(in.rows, in.C)) {
             const unsigned per = kWaveTopThreads / 64;
             hipLaunchKernelGGL(list_waves_kernel<T>, dim3((in.rows + per - 1) / per), dim3(kWaveTopThreads), 0, st, in, set, k, uniform, out);
         } else {
             const int parts = top_parts(in.rows, in.C);
-            uint64_t *keys = (uint64_t *)workspace;
+            uint64_t *keys = (uint64_t *)((char *)workspace + space);
             hipLaunchKernelGGL(list_parts_kernel<T>, dim3(in.rows * parts), dim3(kWaveTopThreads), 0, st, in, set, k, parts, uniform, keys, out);
             if (parts > 1)
                 hipLaunchKernelGGL(list_join_kernel, dim3(in.rows), dim3(kWaveTopThreads), 0, st, in, set, k, parts, uniform, keys, out);
@@ -1328,7 +1591,18 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
         if (!plan.two) break;
         [[fallthrough]];
     }
+    case SPLIT:
     case BLOCKS:
+        if (plan.split) {
+            const int parts = plain_parts(in.rows, in.C), size = plain_part_labels(in.rows, in.C);
+            const SplitSpace ws = {(SplitRow *)workspace, (Part *)((SplitRow *)workspace + in.rows)};
+            const dim3 all(in.rows * parts), one(in.rows), threads(kPlainThreads);
+            hipLaunchKernelGGL(split_largest_kernel<T>, all, threads, 0, st, in, parts, size, ws);
+            hipLaunchKernelGGL(split_histogram_kernel<T>, all, threads, 0, st, in, set, parts, size, ws);
+            hipLaunchKernelGGL(split_sweep_kernel<T>, all, threads, 0, st, in, set, parts, size, ws);
+            hipLaunchKernelGGL(split_pick_kernel<T>, one, threads, 0, st, in, set, k, parts, size, ws, uniform, out);
+            break;
+        }
         if (in.C <= 4096) hipLaunchKernelGGL((sample_blocks_kernel<T, 256>), dim3(in.rows), dim3(256), 0, st, in, set, k, uniform, out);
         else hipLaunchKernelGGL((sample_blocks_kernel<T, 1024>), dim3(in.rows), dim3(1024), 0, st, in, set, k, uniform, out);
     }
@@ -1345,8 +1619,11 @@ size_t mfl_sample_labels_workspace_bytes(int N, int C, int S, int dtype)
     Rows in;
     if (make_rows(in, "", dtype, N, C, S, 0, 1, 0)) return 0;
     size_t most = 0;
-    const Settings sets[2] = {{1.0, 1.0, 0.0, 0, nullptr, nullptr, nullptr, nullptr}, {1.0, 1.0, 0.0, MFL_MAX_TOP_LABELS, nullptr, nullptr, nullptr, nullptr}};
-    for (int i = 0; i < 4; ++i) {
+    // no filters; a short list; top_p; a top_k of every row's own
+    const int some = 0;
+    const Settings sets[4] = {{1.0, 1.0, 0.0, 0, nullptr, nullptr, nullptr, nullptr}, {1.0, 1.0, 0.0, MFL_MAX_TOP_LABELS, nullptr, nullptr, nullptr, nullptr},
+                              {1.0, 0.5, 0.0, 0, nullptr, nullptr, nullptr, nullptr}, {1.0, 1.0, 0.0, 0, nullptr, nullptr, nullptr, &some}};
+    for (int i = 0; i < 8; ++i) {
         in.sc = i & 1 ? 1 : 2;
         const size_t n = plan_of(in, sets[i >> 1]).bytes;
         most = n > most ? n : most;
