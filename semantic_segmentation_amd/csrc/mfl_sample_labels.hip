@@ -299,8 +299,75 @@ template <int K> __device__ inline void draw_by_label(const Best<K> &best, const
     put(out, r, label, log(got / sum));
 }
 
-// The list holds all that top_k leaves, or all labels
-template <typename T, int K>
+// The draw among the labels placed from `cut` on, with the scores read again
+template <typename T>
+__device__ inline void draw_from_cut(const Rows &in, const T *p, double cut, const Weight &weight, double min_p, float u, unsigned r, const Out &out)
+{
+    double sum = 0;
+    auto kept = [&](const float (&x)[8], int c, double (&w)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double v = weight(x[i]);
+            w[i] = c + i < in.C && v >= min_p && place_of(x[i], c + i) >= cut ? v : 0.0;
+        }
+    };
+    for (int c = 0; c < in.C; c += 8) {
+        float x[8];
+        double w[8];
+        load_block(x, p, in.sc, c, in.C);
+        kept(x, c, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += w[i];
+    }
+    const double target = draw_of(u) * sum;
+    double run = 0, got = 0;
+    int label = -1;
+    for (int c = 0; c < in.C; c += 8) {
+        float x[8];
+        double w[8];
+        load_block(x, p, in.sc, c, in.C);
+        kept(x, c, w);
+        int here = -1;
+        double v = 0;
+        pick(w, run, target, here, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) run += w[i];
+        if (here >= 0) label = c + here, got = v;
+        if (here >= 0 && run > target) break;
+    }
+    put(out, r, label, log(got / sum));
+}
+// ... of at most CB labels, in registers
+template <int CB, typename T>
+__device__ inline void draw_from_cut_lone(const Rows &in, const T *p, double cut, const Weight &weight, double min_p, float u, unsigned r, const Out &out)
+{
+    float x[CB];
+    load_block(x, p, in.sc, 0, in.C);
+    double upto[CB], total = 0;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const double v = weight(x[i]);
+        total += i < in.C && v >= min_p && place_of(x[i], i) >= cut ? v : 0.0;
+        upto[i] = total;
+    }
+    const double target = draw_of(u) * total;
+    int label = 0;
+#pragma unroll
+    for (int i = 0; i < CB; ++i) label += upto[i] <= target;
+    if (label >= in.C) {                // past all of it: the last one that weighs something
+        double before = 0;
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            label = upto[i] > before ? i : label;
+            before = upto[i];
+        }
+    }
+    put(out, r, label, log(weight(to_float(p[label * in.sc])) / total));
+}
+
+// The list holds all that top_k leaves, or (ALL) all labels: then the draw follows the scores once more instead of looking for
+// one list entry after the other
+template <typename T, int K, bool ALL>
 __global__ void __launch_bounds__(kLaneThreads)
 list_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out out)
 {
@@ -321,6 +388,15 @@ list_lanes_kernel(Rows in, Settings set, const float *__restrict__ uniform, Out 
         total += w[j];
     }
     const double goal = f.top_p * total;
+    if constexpr (ALL) {
+        double front = 0, cut = best.v[0];
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            cut = w[j] > 0 && (f.top_p >= 1 || front < goal) ? best.v[j] : cut;
+            front += w[j];
+        }
+        return draw_from_cut_lone<K>(in, row.p, cut, weight, f.min_p, u, r, out);
+    }
     double front = 0, sum = 0;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
@@ -392,39 +468,7 @@ __device__ inline void ranked_lane(const Rows &in, const T *p, const Filter &f, 
         front += w;
         return false;
     });
-    double sum = 0;
-    auto kept = [&](const float (&x)[8], int c, double (&w)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double v = weight(x[i]);
-            w[i] = c + i < in.C && v >= f.min_p && place_of(x[i], c + i) >= cut ? v : 0.0;
-        }
-    };
-    for (int c = 0; c < in.C; c += 8) {
-        float x[8];
-        double w[8];
-        load_block(x, p, in.sc, c, in.C);
-        kept(x, c, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += w[i];
-    }
-    const double target = draw_of(u) * sum;
-    double run = 0, got = 0;
-    int label = -1;
-    for (int c = 0; c < in.C; c += 8) {
-        float x[8];
-        double w[8];
-        load_block(x, p, in.sc, c, in.C);
-        kept(x, c, w);
-        int here = -1;
-        double v = 0;
-        pick(w, run, target, here, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) run += w[i];
-        if (here >= 0) label = c + here, got = v;
-        if (here >= 0 && run > target) break;
-    }
-    put(out, r, label, log(got / sum));
+    draw_from_cut(in, p, cut, weight, f.min_p, u, r, out);
 }
 
 template <typename T>
@@ -1554,12 +1598,16 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
         break;
     case LANES: MFL_LANES((plain_lanes_kernel<T>)); break;
     case LIST_LANES:
-        if (k <= 1) MFL_LANES((list_lanes_kernel<T, 1>));
-        else if (k <= 4) MFL_LANES((list_lanes_kernel<T, 4>));
-        else if (k <= 8) MFL_LANES((list_lanes_kernel<T, 8>));
-        else if (k <= 16) MFL_LANES((list_lanes_kernel<T, 16>));
-        else if (k <= 24) MFL_LANES((list_lanes_kernel<T, 24>));
-        else MFL_LANES((list_lanes_kernel<T, 32>));
+        if (in.C <= 32 && k > 4) {
+            if (in.C <= 8) MFL_LANES((list_lanes_kernel<T, 8, true>));
+            else if (in.C <= 16) MFL_LANES((list_lanes_kernel<T, 16, true>));
+            else if (in.C <= 24) MFL_LANES((list_lanes_kernel<T, 24, true>));
+            else MFL_LANES((list_lanes_kernel<T, 32, true>));
+        } else if (k <= 1) MFL_LANES((list_lanes_kernel<T, 1, false>));
+        else if (k <= 4) MFL_LANES((list_lanes_kernel<T, 4, false>));
+        else if (k <= 8) MFL_LANES((list_lanes_kernel<T, 8, false>));
+        else if (k <= 16) MFL_LANES((list_lanes_kernel<T, 16, false>));
+        else MFL_LANES((list_lanes_kernel<T, 32, false>));
         break;
     case ANY_LANES: MFL_LANES((any_lanes_kernel<T>)); break;
 #undef MFL_LANES
