@@ -16,6 +16,13 @@
 // leave nothing but rounding.  Softmax statistics are fp32 as (m, log s) with m the row's largest score, which is exact:
 // differences b_i - Z then lose nothing to the size of the scores.
 //   stats[0] = m,  stats[1] = Z - m / T,  stats[2] = Z_O - Z (0 without rest)
+//
+// Both passes are bound by memory: the forward pass reads the scores, the backward pass reads them again and writes the
+// gradient.  Measured on MI355X, forward / backward: 8 x 21 x 512 x 512 fp32, k = 4 with rest 58 / 96 us (4.5 TB/s each);
+// 2 x 19 x 1024 x 2048 bf16, k = 3 70 / 112 us (3.6 TB/s: two bytes a lane and the vector unit's share); 2048 x 128000 bf16,
+// k = 64 with rest 99 / 207 us (5.3 / 5.1 TB/s: the backward pass starts with the rows that the forward pass read last, part
+// of which is still in the last-level cache, and streams its gradient past it; rows from the first on 316, cached gradient
+// 377 us for both).  16 x 32000: 20 us of kernels in a call that takes the host 100.
 #include "mfl_scores.h"
 
 namespace {

@@ -15,6 +15,13 @@
 // Shapes of work: one lane per row (label maps), one wave or workgroup per row where top_k cuts the row to a short list
 // (mfl_wave_top.h), and one workgroup per row otherwise, which finds the cut by a histogram of the weights.
 //
+// Measured on MI355X.  Lanes: 8 x 21 x 512 x 512 fp32 without filters 60 us (3.5 TB/s; a 64-bit exponential is 17
+// instructions, so the vector unit is about as busy as the memory), top_p alone 216; 2 x 150 x 512 x 512 with top_k 5, top_p
+// and min_p 81 us (3.9 TB/s).  Rows: 1 x 128000 bf16, top_k 50, 21 us and 64 x 50001 f16 without filters 20 us (two launches,
+// latency); 256 x 128000 fp32, every row its own temperature and top_p, 133 us: 25 the largest score (the rate of a copy), 40
+// the histogram (64-bit exponentials and LDS atomics), 43 the sweep, the rest scans and the pick; a binary search over whole
+// passes instead of the histogram took 12.9 ms, a fourth pass for the runs 187 us.
+//
 // A row without a finite largest score (all -inf, or a NaN or +inf among them) has no distribution: label -1, logprob -inf.
 #include "mfl_wave_top.h"
 
@@ -1317,6 +1324,9 @@ plain_pick_kernel(Rows in, Settings set, int parts, int size, const Part *__rest
 }
 
 // ---- few rows of many labels that top_p cuts: the workgroup's steps, spread over the card
+//
+// (1 x 128000 bf16: 47 us against 118 by one workgroup, 64 rows 84 against 124; at 256 rows, one for each CU, 183 against 133,
+// so from kSplitRows on a row gets its workgroup.)
 //
 //   1  the parts' largest scores               2  the histogram: a part's in LDS, then added to the row's (integers)
 //   3  every workgroup finds the row's bin for itself; its part's sure weights summed, the bin's labels listed

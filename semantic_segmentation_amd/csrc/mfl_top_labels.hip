@@ -10,6 +10,11 @@
 //           off the list's end can no longer be among the k best and goes into the rest's running sum, so one pass gives
 //           both and the rest is never a difference of two sums.
 //   rows    one or more waves per row, for rows of many labels (mfl_wave_top.h).
+//
+// Measured on MI355X.  Lanes, 8 x 21 x 512 x 512 fp32, k = 4: 51 us, 4.9 TB/s, the rate of a large copy; 4 x 150 x 512 x 512,
+// k = 8: 164 us, 4.3 TB/s (the list as separate words for score and label: 198 us, bound by the vector unit).  Rows,
+// 1024 x 32001 bf16, k = 64: 36 us, 1.8 TB/s, bound by the vector unit (about 20 instructions a score, 9 of them the rest's
+// exponential and sum).
 #include "mfl_wave_top.h"
 
 namespace {
