@@ -652,7 +652,8 @@ list_join_kernel(Rows in, Settings set, int k, int parts, const float *__restric
 //      rows): counts, and masses as 64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose sums do not depend on the
 //      order of the atomics; running sums over the bins name the bin that the cut falls into
 //   3  that bin's labels, a list in LDS; every one counts what lies above it in the list, and the lowest that stays is the
-//      cut.  (A bin of more labels than the list holds, all of nearly one score: a binary search over the rank keys.)  On the
+//      cut.  (A bin of more labels than the list holds: where they share one score, counted along the row, else a
+//      binary search over the rank keys.)  On the
 //      way the weights above the bin are summed in runs of neighbouring labels
 //   4  the run that the draw falls into, and the label in it
 //
@@ -906,6 +907,63 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
         __syncthreads();
     }
 
+    // How many labels of `each` reach the goal from front on
+    MFL_INLINE unsigned long long share_of(double goal, unsigned long long front, unsigned long long each) const
+    {
+        unsigned long long n = (unsigned long long)fmax(1.0, __builtin_ceil((goal - (double)front) / (double)each));
+        while (n > 1 && (double)(front + (n - 1) * each) >= goal) --n;
+        while (n < (unsigned long long)C && (double)(front + n * each) < goal) ++n;
+        return n;
+    }
+    // The rank key of the n-th label of one score, in label order (of the last one, if there are fewer)
+    MFL_INLINE uint64_t nth_of_score(float score, unsigned long long n)
+    {
+        sum_runs([&](const float (&x)[V], int c) __attribute__((always_inline)) {
+            double found = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) found += x[i] == score && c + i < C ? 1.0 : 0.0;
+            return found;
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int lane = threadIdx.x;
+            double left = (double)n;
+            int run = 0, label = -1;
+            for (; run < count_runs - 1 && sh.runs[run] < left; ++run) left -= sh.runs[run];
+            for (int t = run * per; t < min(tiles, (run + 1) * per); ++t) {
+                float x[V];
+                load_tile(x, t);
+                const int c = t * step + lane * V;
+                int own = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) own += x[i] == score && c + i < C;
+                int upto = own;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int other = __shfl_up(upto, o);
+                    if (lane >= o) upto += other;
+                }
+                const uint64_t past = __ballot(own > 0 && upto >= left), holds = __ballot(own > 0);
+                if (holds) {
+                    const int who = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)holds);
+                    int at = upto - own, l = -1;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const bool here = x[i] == score && c + i < C && !(l >= 0 && at >= left);
+                        at += here;
+                        l = here ? c + i : l;
+                    }
+                    label = __shfl(l, who);
+                }
+                if (past) break;
+                left -= __shfl(upto, 63);
+            }
+            if (lane == 0) sh.low_key = rank_key(score_key(score), label);
+        }
+        __syncthreads();
+        return sh.low_key;
+    }
+
     // The lowest rank key that top_k and top_p keep (0: all); sh.runs becomes the runs' kept weights
     MFL_INLINE uint64_t cut_of(const Filter &f)
     {
@@ -957,6 +1015,7 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
             __syncthreads();
             bin = sh.bin;
             front = sh.bin_front;
+            __syncthreads();
             sure = lowest_of(bin - 1);
             open = lowest_of(bin);
             sweep<true>(sure, open, cut, f.min_p);
@@ -986,11 +1045,32 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
                     summed = true;
                 }
             } else {
-                // the largest key from which on at least `goal` is held
+                // the largest key from which on at least `goal` is held, bit by bit where the bin's keys differ
+                if (threadIdx.x == 0) sh.low_key = ~0ull, sh.bin_front = 0;
+                __syncthreads();
+                unsigned long long every = ~0ull, any = 0;
+                each([&](float x, int c) __attribute__((always_inline)) {
+                    const uint64_t key = rank_key(score_key(x), c);
+                    if (bin_of(x) != bin || key < cut) return;
+                    every &= key;
+                    any |= key;
+                });
+                atomicAnd(&sh.low_key, every);
+                atomicOr(&sh.bin_front, any);
+                __syncthreads();
+                every = sh.low_key;
+                any = sh.bin_front;
                 uint64_t best = 0;
+                const bool one_score = every >> 32 == any >> 32;
+                if (one_score) best = nth_of_score(rank_score(any), share_of(goal, front, count ? 1 : mass(rank_score(any))));
 #pragma unroll 1
-                for (int b = 63; b >= 0; --b) {
+                for (int b = one_score ? -1 : 63; b >= 0; --b) {
+                    if (!(any >> b & 1)) continue;
                     const uint64_t at = best | 1ull << b, from = at > cut ? at : cut;
+                    if (every >> b & 1) {
+                        best = at;
+                        continue;
+                    }
                     unsigned long long held = 0;
                     each([&](float x, int c) __attribute__((always_inline)) {
                         if (bin_of(x) == bin && rank_key(score_key(x), c) >= from) held += count ? 1 : mass(x);

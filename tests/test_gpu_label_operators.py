@@ -333,7 +333,7 @@ def test_sample_labels_with_settings_of_every_row(shape, S):
     check_sample(S, x, u, top_k=k)
 
 
-@pytest.mark.parametrize("C", [8, 100, 600, 5000])
+@pytest.mark.parametrize("C", [8, 100, 600, 5000, 30000])
 def test_sample_labels_of_equal_masked_and_unusual_scores(C, S):
     low = torch.finfo(torch.float32).min
     x = torch.zeros(10, C, device="cuda")
@@ -352,6 +352,14 @@ def test_sample_labels_of_equal_masked_and_unusual_scores(C, S):
                dict(min_p=0.3, temperature=0.5)):
         check_sample(S, x, u, **kw)
         check_sample(S, x.reshape(5, 2, C).movedim(2, 1), u.reshape(5, 2), **kw)
+    # a long run of one score that the cut falls into, in front of and behind others
+    z = torch.zeros(4, C, device="cuda")
+    z[0, : C // 5] = 1.0
+    z[1, C // 3:] = -2.0
+    z[2, ::3] = 0.5
+    z[3, 1::7] = -INF
+    for kw in (dict(top_p=0.7), dict(top_k=C // 2), dict(top_k=max(2, C // 2), top_p=0.9), dict(top_p=0.95, min_p=0.3), dict(top_k=C // 5 + 1)):
+        check_sample(S, z, u[1:5].contiguous(), **kw)
     # numbers outside [0, 1): the first and the last kept label
     odd = torch.tensor([-1.0, 1.0, 2.0, float("nan")], device="cuda")
     y = torch.zeros(4, C, device="cuda")
