@@ -217,6 +217,7 @@ def top_labels(scores: torch.Tensor, k: int, temperature: float = 1.0):
     (values [N, k, ...] of the scores' type, labels [N, k, ...] int32, rest [N, ...] float32), with rest = log sum
     exp(score / temperature) over all other labels (-inf if there are none).  The record distillation_forward reads."""
     v, args = _score_rows(scores)
+    k = int(k)
     if not 1 <= k <= min(args[3], _lib.MAX_TOP_LABELS):
         raise ValueError(f"k must be between 1 and min(C, {_lib.MAX_TOP_LABELS}), got {k} with C = {args[3]}")
     shape, device = tuple(scores.shape), scores.device
@@ -225,7 +226,7 @@ def top_labels(scores: torch.Tensor, k: int, temperature: float = 1.0):
     rest = torch.empty((shape[0],) + shape[2:], dtype=torch.float32, device=device)
     n = lib.mfl_top_labels_workspace_bytes(*args[2:5], args[1], k)
     ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    _lib.call_scores(lib.mfl_top_labels, "mfl_top_labels", v, *args, temperature, k, values.data_ptr(), labels.data_ptr(),
+    _lib.call_scores(lib.mfl_top_labels, "mfl_top_labels", v, *args, float(temperature), k, values.data_ptr(), labels.data_ptr(),
                      rest.data_ptr(), _address(ws), n)
     return values, labels, rest
 
@@ -252,7 +253,7 @@ def _distillation_forward(scores, v, args, record, rows, temperature):
     stats = torch.empty((5,) + rows, dtype=torch.float32, device=scores.device)
     n = lib.mfl_distillation_workspace_bytes(*args[2:5], args[1], record[5])
     ws = torch.empty(n, dtype=torch.uint8, device=scores.device) if n else None
-    _lib.call_scores(lib.mfl_distillation_forward, "mfl_distillation_forward", v, *args, *record, temperature, loss.data_ptr(),
+    _lib.call_scores(lib.mfl_distillation_forward, "mfl_distillation_forward", v, *args, *record, float(temperature), loss.data_ptr(),
                      stats.data_ptr(), _address(ws), n)
     return loss, stats
 
@@ -263,7 +264,7 @@ def _distillation_backward(scores, v, args, record, stats, grad_loss, temperatur
     if out[0] != grad.data_ptr():                          # (a layout without one common stride)
         grad = torch.empty_like(scores, memory_format=torch.contiguous_format, requires_grad=False)
         g, out = _score_rows(grad, "the gradient")
-    _lib.call_scores(lib.mfl_distillation_backward, "mfl_distillation_backward", v, *args, *record, temperature, stats.data_ptr(),
+    _lib.call_scores(lib.mfl_distillation_backward, "mfl_distillation_backward", v, *args, *record, float(temperature), stats.data_ptr(),
                      grad_loss.data_ptr(), out[0], *out[5:])
     return grad
 
@@ -317,7 +318,7 @@ def sample_labels(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
                 raise ValueError(f"top_k must not be negative, got {x}")
             settings += [min(int(x), 0x7fffffff), None]
         else:
-            settings += [x, None]
+            settings += [float(x), None]
     labels = torch.empty(rows, dtype=dtype, device=scores.device)
     logprob = torch.empty(rows, dtype=torch.float32, device=scores.device) if want_logprob else None
     n = lib.mfl_sample_labels_workspace_bytes(*args[2:5], args[1])

@@ -382,6 +382,33 @@ def test_sample_labels_types_and_void(S):
     assert int(S.ops.iou_counts(greedy, greedy, 21)[1].sum()) == greedy.numel() - 1
 
 
+def test_refusals_and_numbers_of_other_types(S):
+    """Wrong companions are refused before a launch; numpy's numbers serve like Python's."""
+    x = scores_of((4, 30, 5), torch.float32, 78)
+    u = torch.rand(4, 5, generator=gen(79), device="cuda")
+    values, labels, rest = S.ops.top_labels(x, np.int64(3), temperature=np.float32(1.5))
+    assert all(torch.equal(a, b) for a, b in zip((values, labels, rest), S.ops.top_labels(x, 3, 1.5)))
+    assert torch.equal(S.ops.sample_labels(x, u, top_k=np.int32(4), top_p=np.float32(0.5)), S.ops.sample_labels(x, u, top_k=4, top_p=0.5))
+    assert torch.equal(S.ops.sample_labels(x, u, top_k=1 << 40), S.ops.sample_labels(x, u))
+    for call, kind in [(lambda: S.ops.top_labels(x, 0), ValueError), (lambda: S.ops.top_labels(x, 31), ValueError),
+                       (lambda: S.ops.top_labels(x, 3, 0.0), ValueError), (lambda: S.ops.top_labels(x.double(), 3), RuntimeError),
+                       (lambda: S.ops.top_labels(x[0, 0], 1), RuntimeError), (lambda: S.ops.top_labels(x[:0], 1), RuntimeError),
+                       (lambda: S.ops.sample_labels(x, u[:, :4]), RuntimeError), (lambda: S.ops.sample_labels(x, u.double()), RuntimeError),
+                       (lambda: S.ops.sample_labels(x, u.cpu()), RuntimeError), (lambda: S.ops.sample_labels(x, u, top_k=-1), ValueError),
+                       (lambda: S.ops.sample_labels(x, u, top_p=0.0), ValueError), (lambda: S.ops.sample_labels(x, u, min_p=1.5), ValueError),
+                       (lambda: S.ops.sample_labels(x, u, temperature=-1.0), ValueError), (lambda: S.ops.sample_labels(x, u, dtype=torch.int16), TypeError),
+                       (lambda: S.ops.sample_labels(x, u, temperature=torch.ones(3, device="cuda")), RuntimeError),
+                       (lambda: S.ops.sample_labels(x, u, top_k=torch.ones(4, device="cuda")), RuntimeError),
+                       (lambda: S.ops.distillation_forward(x, values, labels.long(), rest), RuntimeError),
+                       (lambda: S.ops.distillation_forward(x, values[:, :2], labels, rest), RuntimeError),
+                       (lambda: S.ops.distillation_forward(x, values, labels, rest[:2]), RuntimeError),
+                       (lambda: S.ops.distillation_forward(x, values, labels, rest, valid=rest), RuntimeError),
+                       (lambda: S.ops.distillation_forward(x, values[..., 0], labels, rest), RuntimeError),
+                       (lambda: S.training.distillation_loss(x, values.requires_grad_(True), labels), RuntimeError)]:
+        with pytest.raises(kind):
+            call()
+
+
 def test_sampled_shares_follow_the_distribution(S):
     """An even grid of draws: every label gets its share of it, to within the two ends of its interval."""
     n, C = 4096, 37
