@@ -649,12 +649,11 @@ list_join_kernel(Rows in, Settings set, int k, int parts, const float *__restric
 //
 //   1  the largest score
 //   2  where top_k or top_p cut: a histogram over 4096 bins of (largest - score) / T, 128 a unit (a quarter of that for short
-//      rows): counts, and masses as 64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose sums do not depend on the
-//      order of the atomics; running sums over the bins name the bin that the cut falls into
+//      rows): counts, and masses as 64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose
+//      sums do not depend on the order of the atomics; running sums over the bins name the bin that the cut falls into
 //   3  that bin's labels, a list in LDS; every one counts what lies above it in the list, and the lowest that stays is the
-//      cut.  (A bin of more labels than the list holds: where they share one score, counted along the row, else a
-//      binary search over the rank keys.)  On the
-//      way the weights above the bin are summed in runs of neighbouring labels
+//      cut.  (A bin of more labels than the list holds: where they share one score, counted along the row, else a binary
+//      search over the rank keys.)  On the way the weights above the bin are summed in runs of neighbouring labels
 //   4  the run that the draw falls into, and the label in it
 //
 // Steps 2 and 3 read the row again, from the caches if it fits; scores below the cut cost a compare in step 3.

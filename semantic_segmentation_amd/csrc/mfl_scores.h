@@ -237,7 +237,6 @@ __device__ inline float log_of(LogSum a, float inv_t)
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
 constexpr double kLog2eD = 1.44269504088896340736;
 
 // (log2(e) / temperature and its inverse have to be ordinary fp32 numbers)
