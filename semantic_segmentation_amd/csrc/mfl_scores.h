@@ -222,11 +222,13 @@ __device__ inline float minus_inf_where(uint32_t mask, int i, float x)
     return __builtin_bit_cast(float, (m & (int)0xff800000) | (~m & __builtin_bit_cast(int, x)));
 }
 
-// log(1 + s) for s >= -1 to a few steps: log(u) of the rounded u = 1 + s, scaled by the part of s that u keeps (Kahan)
+// log(1 + s) for s >= -1 to a few steps: log(u) of the rounded u = 1 + s, scaled by the part of s that u keeps (Kahan).  From
+// 2^24 on u is s to half a step, and the part is not looked at: the reciprocal of a number above 2^126 is flushed to zero.
 __device__ inline float log_1p(float s)
 {
     const float u = 1.f + s, kept = u - 1.f;
-    return kept == 0.f || u == INFINITY ? s : logf(u) * (s * __builtin_amdgcn_rcpf(kept));
+    if (kept == 0.f) return s;
+    return s < 0x1p24f ? logf(u) * (s * __builtin_amdgcn_rcpf(kept)) : logf(u);
 }
 
 // log(s * exp(m / temperature)); -inf for nothing, and an infinite score stays infinite

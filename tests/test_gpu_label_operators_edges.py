@@ -1,0 +1,52 @@
+"""GPU tests of the label-selection operators where fp32 runs out: rows that are not numbers, gaps near the ends of the
+fp32 exponent, masses far below the largest, bins of the cut that overflow their list, calls of very many rows.  The plain
+64-bit restatements, the tolerances and their derivation are those of test_gpu_label_operators.py."""
+import numpy as np
+import pytest
+import torch
+
+import label_reference as R
+import test_gpu_label_operators as G
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module")
+def S():
+    import semantic_segmentation_amd as S
+    assert torch.cuda.is_available(), "GPU tests need a ROCm device"
+    return S
+
+
+def lay(x, planes):
+    """[rows, C] as a matrix, or as class planes of two images"""
+    return x if not planes else x.reshape(2, x.shape[0] // 2, x.shape[1]).movedim(2, 1).contiguous()
+
+
+def lay_rows(x, planes):
+    return x if not planes else x.reshape(2, -1)
+
+
+# ------------------------------------------------------------------ distillation
+
+GAPS = [80.0, 86.9, 87.2, 87.4, 88.0, 88.4, 88.6, 88.75, 89.0, 95.0, 104.0]
+
+
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("C", [12, 24, 60, 900])
+def test_distillation_of_gaps_near_the_end_of_the_exponent(C, planes, S):
+    """Record and rest exp(gap) apart, on the student's side, on the teacher's, and on both: ratios around 2^126 and 2^128."""
+    k = 3
+    pairs = [(s, t) for s in [0.5, -1.0] + GAPS + [-g for g in GAPS] for t in [0.7] + GAPS + [-g for g in GAPS]]
+    pairs += pairs[:len(pairs) % 2]                        # (an even number of rows)
+    x = G.scores_of((len(pairs), C), torch.float32, 201, 0.5)
+    labels = torch.rand(x.shape, generator=G.gen(202), device="cuda").argsort(1)[:, :k].to(torch.int32).contiguous()
+    own = torch.gather(x, 1, labels.long())
+    others = torch.logsumexp(x.scatter(1, labels.long(), -INF), 1, keepdim=True)
+    student = torch.tensor([s for s, _ in pairs], device="cuda").unsqueeze(1)
+    x.scatter_(1, labels.long(), own - torch.logsumexp(own, 1, keepdim=True) + others + student)
+    values = G.scores_of((len(pairs), k), torch.float32, 203, 0.5)
+    rest = torch.logsumexp(values, 1) - torch.tensor([t for _, t in pairs], device="cuda")
+    G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), lay_rows(rest, planes), 1.0)
