@@ -90,6 +90,8 @@ __device__ inline Stats stats_of(Excess top, LogSum out, const Teacher &t)
 {
     const Excess all = join(top, Excess{out.m, out.s - 1.f}, t.c2);
     if (all.m == -INFINITY && all.s == -1.f) return kNoStats;
+    // (a NaN score is in the sum, whatever the largest score came to without it)
+    if (all.s != all.s) return {NAN, NAN, NAN, NAN, NAN, NAN};
     Stats a = {all.m, log_1p(all.s), -INFINITY, 0.f, -INFINITY, all.s};
     if (out.m == -INFINITY && out.s == 0.f) return a;
     a.mo = out.m;

@@ -50,3 +50,28 @@ def test_distillation_of_gaps_near_the_end_of_the_exponent(C, planes, S):
     values = G.scores_of((len(pairs), k), torch.float32, 203, 0.5)
     rest = torch.logsumexp(values, 1) - torch.tensor([t for _, t in pairs], device="cuda")
     G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), lay_rows(rest, planes), 1.0)
+
+
+@pytest.mark.parametrize("dtype", G.DTYPES)
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("C", [3, 21, 60, 900])
+def test_distillation_of_rows_that_are_no_numbers(C, planes, dtype, S):
+    """A NaN among a valid row's scores makes its loss and its whole gradient NaN, whatever else stands there: a student that
+    has diverged must not look like one that has nothing to learn."""
+    x = G.scores_of((8, C), torch.float32, 211)
+    values = G.scores_of((8, 2), torch.float32, 212).to(dtype)
+    labels = torch.tensor([[0, 2]] * 8, dtype=torch.int32, device="cuda")
+    rest = torch.zeros(8, device="cuda")
+    x[0] = NAN
+    x[1] = -INF
+    x[1, 1] = NAN                                          # outside the record
+    x[2] = -INF
+    x[2, 2] = NAN                                          # in it
+    x[3, 1:] = NAN
+    x[4, 0] = NAN
+    x[5] = -INF                                            # nothing, but nothing wrong: 0
+    x = x.to(dtype)
+    for r in (rest, None):
+        G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), 1.5)
+        loss, _ = S.ops.distillation_forward(lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), 1.5)
+        assert torch.isnan(loss.reshape(-1)).tolist() == [True] * 5 + [False] * 3 and float(loss.reshape(-1)[5]) == 0
