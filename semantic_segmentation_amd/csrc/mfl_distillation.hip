@@ -59,6 +59,7 @@ __device__ inline Target target_of(const Teacher &t, Excess sum, bool named, flo
     g.any = named && !(sum.m == -INFINITY && sum.s == -1.f);
     const float ratio = (1.f + sum.s) * __builtin_amdgcn_exp2f(-above * kLog2e);        // the record next to the rest
     g.log_p_rest = rest == -INFINITY ? -INFINITY : ratio == INFINITY ? above - g.l : -log_1p(ratio);
+    if (g.s != g.s) g.log_p_rest = NAN;         // (a NaN among the values leaves no share a number, an empty rest's neither)
     g.p_rest = __builtin_amdgcn_exp2f(g.log_p_rest * kLog2e);
     return g;
 }
@@ -141,7 +142,7 @@ __device__ inline Slope slope_of(const Stats &a, const Teacher &t, const Target 
 // taken: the record's share of the label, -1 where it is not named
 __device__ inline float slope(const Slope &s, float x, float taken, float c2)
 {
-    const bool named = taken >= 0.f;
+    const bool named = !(taken < 0.f);          // (a share may be NaN)
     const float e = __builtin_amdgcn_exp2f((x - (named ? s.m_top : s.m_out)) * c2 + (named ? s.o_top : s.o_out));
     return named ? s.up * (e - taken) : s.f_out * e;
 }
@@ -376,7 +377,7 @@ backward_lanes_kernel(Rows in, Teacher t, const float *__restrict__ stats, const
         for (int i = 0; i < CB; ++i) {
             const float share = taken[i][threadIdx.x];
             if (i < SURE || c0 + i < in.C) store_once(slope(sl, x[i], share, t.c2), w + i * gc);
-            if (share >= 0.f) taken[i][threadIdx.x] = -1.f;
+            if (!(share < 0.f)) taken[i][threadIdx.x] = -1.f;
         }
     }
 }

@@ -75,3 +75,24 @@ def test_distillation_of_rows_that_are_no_numbers(C, planes, dtype, S):
         G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), 1.5)
         loss, _ = S.ops.distillation_forward(lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), 1.5)
         assert torch.isnan(loss.reshape(-1)).tolist() == [True] * 5 + [False] * 3 and float(loss.reshape(-1)[5]) == 0
+
+
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("C", [3, 21, 60, 900])
+def test_distillation_of_records_that_are_no_numbers(C, planes, S):
+    """A NaN among the teacher's values, or a rest that is one, reaches every label whose gradient it enters: the record's
+    labels, and with rest all others."""
+    x = G.scores_of((6, C), torch.float32, 221)
+    values = G.scores_of((6, 3), torch.float32, 222)
+    labels = torch.tensor([[0, 2, 1]] * 6, dtype=torch.int32, device="cuda")
+    rest = torch.zeros(6, device="cuda")
+    values[0, 1] = NAN
+    values[1] = NAN
+    values[2], values[2, 0] = -INF, NAN
+    values[3, 2], labels[3, 2] = NAN, -1                   # of no class: passed over
+    labels[4, 1], values[4, 1] = 0, NAN                    # a label named twice
+    for r in (rest, torch.full_like(rest, -INF), None):
+        G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), 1.5)
+    values = G.scores_of((6, 3), torch.float32, 223)
+    rest[1::2] = NAN
+    G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), lay_rows(rest, planes), 1.5)
