@@ -167,7 +167,8 @@ template <int K> struct Best {
     }
 };
 
-// (m, s) stands for s * exp(m): running maximum and sum.  m = -inf: nothing yet.
+// (m, s) stands for s * exp(m): running maximum and sum.  m = -inf: nothing yet; m = NaN: a NaN was among them (an infinite
+// score makes s NaN as well, so s alone cannot tell).
 struct LogSum {
     float m, s;
 };
@@ -175,12 +176,12 @@ __device__ inline float finite_or_zero(float m) { return m == -INFINITY ? 0.f : 
 // both in units of scores; c = log2(e) / temperature
 __device__ inline LogSum join(LogSum a, LogSum b, float c)
 {
-    const float m = fmaxf(a.m, b.m), r = finite_or_zero(m);
+    const float m = max_or_nan(a.m, b.m), r = finite_or_zero(m);
     return {m, a.s * __builtin_amdgcn_exp2f((a.m - r) * c) + b.s * __builtin_amdgcn_exp2f((b.m - r) * c)};
 }
 __device__ inline void add_score(LogSum &a, float v, float c)
 {
-    const float m = fmaxf(a.m, v), r = finite_or_zero(m);
+    const float m = max_or_nan(a.m, v), r = finite_or_zero(m);
     a.s = a.s * __builtin_amdgcn_exp2f((a.m - r) * c) + __builtin_amdgcn_exp2f((v - r) * c);
     a.m = m;
 }
@@ -231,7 +232,7 @@ __device__ inline float log_1p(float s)
     return s < 0x1p24f ? logf(u) * (s * __builtin_amdgcn_rcpf(kept)) : logf(u);
 }
 
-// log(s * exp(m / temperature)); -inf for nothing, and an infinite score stays infinite
+// log(s * exp(m / temperature)); -inf for nothing, an infinite score stays infinite and a NaN a NaN
 __device__ inline float log_of(LogSum a, float inv_t)
 {
     if (a.m == INFINITY) return INFINITY;

@@ -45,7 +45,7 @@ top_lanes_kernel(Rows in, float c2, float inv_t, int k, T *__restrict__ values, 
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             x[i] = place_score(best.insert(place_of(to_float(raw[i]), c + i)));
-            m = fmaxf(m, x[i]);
+            m = max_or_nan(m, x[i]);
         }
         const float ref = finite_or_zero(m);
         float t = sum.s * __builtin_amdgcn_exp2f((sum.m - ref) * c2);

@@ -137,7 +137,7 @@ template <bool REST> struct WaveTop {
     {
         float top = rest.m;
 #pragma unroll
-        for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
+        for (int i = 0; i < V; ++i) top = max_or_nan(top, x[i]);
         const float ref = finite_or_zero(top);
         float sum = 0.f;
 #pragma unroll

@@ -96,3 +96,20 @@ def test_distillation_of_records_that_are_no_numbers(C, planes, S):
     values = G.scores_of((6, 3), torch.float32, 223)
     rest[1::2] = NAN
     G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), lay_rows(rest, planes), 1.5)
+
+
+# ------------------------------------------------------------------ top labels
+
+@pytest.mark.parametrize("C,k", [(40, 3), (300, 3), (700, 20), (9000, 3), (9000, 100)])
+def test_rest_of_rows_that_are_no_numbers(C, k, S):
+    """More NaN than the record holds, next to infinities: the rest is no number either."""
+    x = G.scores_of((6, C), torch.float32, 271)
+    x[0, : k + 2] = NAN
+    x[0, k + 2:k + 4] = INF
+    x[1, C - k - 5:] = NAN
+    x[1, 0] = INF
+    x[2] = NAN
+    x[3], x[3, ::2] = -INF, NAN
+    x[4, : k + 1], x[4, k + 1] = INF, -INF                 # infinities alone: an infinite rest
+    for y in (x, x.reshape(2, 3, C).movedim(2, 1)):
+        G.check_top(S, y, k, 1.0)
