@@ -387,7 +387,9 @@ int mfl_distillation_backward(const void *scores, int dtype, int N, int C, int S
  * follows the marginals).  With w = exp((score - largest) / T) and the labels ranked as in mfl_top_labels: keep the
  * first top_k; of those the ones in front of which less than top_p of their mass lies; of those the ones with
  * w >= min_p (the first always stays).  labels = the first kept label, in label order, whose running sum exceeds
- * uniform * (kept mass); logprob = log of its share of that mass.  Sums are 64-bit.
+ * uniform * (kept mass); logprob = log of its share of that mass.  Weights and sums are 64-bit floats; where top_p cuts a
+ * long row without a short top_k, the mass in front of a label is summed from integers, each weight rounded to a part in
+ * 2^min(51, 62 - b) of itself, b the bits of C: 2^45 at C = 128 000, 2^31 at 2^30.
  *   uniform: [N][S] in [0, 1) (below: 0; 1 and above: the last kept label)
  *   temperature (0: the largest score), top_k (0: all), top_p in (0, 1], min_p in [0, 1]: each for all rows, or, where
  *   the array next to it is not NULL, [N] values of which temperature <= 0, top_k <= 0, top_p >= 1, min_p <= 0 mean the

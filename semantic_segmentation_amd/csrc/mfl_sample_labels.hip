@@ -9,7 +9,9 @@
 // The order of label numbers, not of scores, is what the running sum follows: without filters nothing has to be sorted.
 //
 // All weights and sums are 64-bit floats: a label's border in a row of 10^5 labels is 10^-5 of the mass wide, so fp32
-// sums (10^-7) would misplace about one draw in a hundred, and a batch of maps has millions of draws.
+// sums (10^-7) would misplace about one draw in a hundred, and a batch of maps has millions of draws.  The masses of a
+// histogram are integers, a label's rounded to a part in 2^min(51, 62 - bits of C) of itself (2^45 at 128 000 labels, 2^31
+// at the most that a call takes), however far below the largest weight it lies (Bins).
 //
 // Settings may differ from n to n (arrays of N).  T <= 0 takes the largest; top_k <= 0, top_p >= 1 and min_p <= 0 keep all.
 // Shapes of work: one lane per row (label maps), one wave or workgroup per row where top_k cuts the row to a short list
@@ -649,8 +651,8 @@ list_join_kernel(Rows in, Settings set, int k, int parts, const float *__restric
 //
 //   1  the largest score
 //   2  where top_k or top_p cut: a histogram over 4096 bins of (largest - score) / T, 128 a unit (a quarter of that for short
-//      rows): counts, and masses as 64-bit fixed point (2^51 or less for the largest weight, so that C of them fit), whose
-//      sums do not depend on the order of the atomics; running sums over the bins name the bin that the cut falls into
+//      rows): counts, and masses as 64-bit fixed point (2^51 or less for a bin's own largest weight, so that C of them fit),
+//      whose sums do not depend on the order of the atomics; running sums over the bins name the bin that the cut falls into
 //   3  that bin's labels, a list in LDS; every one counts what lies above it in the list, and the lowest that stays is the
 //      cut.  (A bin of more labels than the list holds: where they share one score, counted along the row, else a binary
 //      search over the rank keys.)  On the way the weights above the bin are summed in runs of neighbouring labels
@@ -699,6 +701,39 @@ template <typename V, int NT> __device__ inline V block_front(V v, V *part, V &a
     return before + (lane ? ahead : V(0));
 }
 
+// The bin in which a running sum over all threads' bins reaches the goal, and what is left of the goal there.  A thread has n
+// bins, held(0) .. held(n - 1), with `front` in front of them.  (Sums of doubles, each rounded by itself: where they leave a
+// gap at the goal, the next bin that holds something, or the last, has it.)  first = ~0 and last = 0 before, with a barrier
+// between; some bin holds something.
+struct Reach {
+    unsigned first, last;
+    int bin;
+    double left;
+};
+template <typename F> MFL_INLINE void find_bin(int n, double front, double mine, double goal, F held, Reach &sh)
+{
+    const uint64_t holds = __ballot(mine > 0), past = __ballot(mine > 0 && front + mine >= goal);
+    if ((threadIdx.x & 63) == 0) {
+        if (past) atomicMin(&sh.first, threadIdx.x + __ffsll((unsigned long long)past) - 1);
+        if (holds) atomicMax(&sh.last, threadIdx.x + 63 - __clzll((long long)holds));
+    }
+    __syncthreads();
+    if (threadIdx.x == (sh.first != ~0u ? sh.first : sh.last)) {
+        int at = -1;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const double here = held(i);
+            if (here > 0 && (at < 0 || front < goal)) {
+                at = i;
+                sh.left = goal - front;
+            }
+            front += here;
+        }
+        sh.bin = threadIdx.x * n + max(at, 0);
+    }
+    __syncthreads();
+}
+
 // What the listed keys above one hold.  The list ends in zeros up to a multiple of eight, so that eight are on their way at once.
 MFL_INLINE unsigned long long held_above(const unsigned long long *keys, const unsigned long long *masses, int n, uint64_t key)
 {
@@ -710,12 +745,19 @@ MFL_INLINE unsigned long long held_above(const unsigned long long *keys, const u
     return above;
 }
 
-// Bins of (largest - score) / T and fixed-point masses of a row
+// Bins of (largest - score) / T and fixed-point masses of a row.  A bin's weights are at most 2^-edge(bin); its masses are
+// integers in steps of 2^-(bits + edge(bin)).  (One step for all bins, next to the row's largest weight, would leave nothing of
+// a tail that may hold 10^-7 of the mass at 10^6 labels, where draws are 2^-24 apart.)
 template <int BINS> struct Bins {
     static constexpr int kBins = BINS;
     float m, scale;
     Weight weight;
-    int bits;                   // of the masses
+    int bits;                   // of the largest mass
+
+    // (a bin's log2(e) units in 2^-19, rounded down by 5 10^-6 of itself or more: bin_of is off by 2 10^-7 at most)
+    static constexpr uint32_t kBinEdge = (uint32_t)(kUnits / BINS * kLog2eD * (1 << 19));
+    MFL_INLINE static int edge(int bin) { return (int)(__umul24((uint32_t)bin, kBinEdge) >> 19); }
+    MFL_INLINE double unit(int bin) const { return __builtin_ldexp(1.0, -bits - edge(bin)); }
 
     MFL_INLINE explicit Bins(int C)
     {
@@ -729,10 +771,10 @@ template <int BINS> struct Bins {
         weight = {m, f.inv_t * kLog2eD};
     }
     MFL_INLINE int bin_of(float x) const { return min((int)((m - x) * scale), BINS - 1); }
-    MFL_INLINE uint64_t mass(float x) const
+    MFL_INLINE uint64_t mass(float x, int bin) const
     {
         // 2^52 + an integer below 2^52: the low bits of the sum are that integer
-        const double v = __builtin_ldexp(weight(x), bits) + 4503599627370496.0;
+        const double v = weight.scaled(x, bits + edge(bin)) + 4503599627370496.0;
         return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
     }
     // The lowest score of bins 0 .. b (they grow as the score falls); b = -1: none
@@ -757,10 +799,10 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
     using Bins<4 * NT>::kBins;
     using Bins<4 * NT>::m;
     using Bins<4 * NT>::weight;
-    using Bins<4 * NT>::bits;
     using Bins<4 * NT>::bin_of;
     using Bins<4 * NT>::mass;
     using Bins<4 * NT>::lowest_of;
+    using Bins<4 * NT>::unit;
     static constexpr int V = kVec<T>, step = 64 * V, waves = NT / 64;
     struct Shared {
         uint32_t counts[kBins];
@@ -770,9 +812,10 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
         unsigned long long more[kRuns];         // fixed point
         unsigned long long upart[NT / 64];
         double dpart[NT / 64];
+        Reach reach;
         float fpart[NT / 64];
         unsigned listed, bin;
-        unsigned long long bin_front, low_key;
+        unsigned long long low_key, any_key;
     };
     Shared &sh;
     const T *p;
@@ -839,12 +882,11 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
             for (int i = 0; i < V; ++i) x[i] = c + i < C ? to_float(p[(c + i) * sc]) : -INFINITY;
         }
     }
-    // sh.runs = sums of f(vector, its first label) over the runs.  A wave takes four runs at a time, to have four loads in
-    // flight.  f is called by whole waves.
-    template <typename F> MFL_INLINE void sum_runs(F f)
+    // sh.runs = sums of f(vector, its first label) over the runs.  A wave takes U runs at a time, to have U loads in flight.
+    // f is called by whole waves.
+    template <int U, typename F> MFL_INLINE void sum_runs(F f)
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        constexpr int U = 4;
 #pragma unroll 1
         for (int e = wave; e < count_runs; e += U * waves) {
             double sum[U] = {};
@@ -874,7 +916,7 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
     // whose key is at least cut; with LIST those labels between are listed
     template <bool LIST> MFL_INLINE void sweep(float sure, float open, uint64_t cut, double min_p)
     {
-        sum_runs([&](const float (&x)[V], int c) __attribute__((always_inline)) {
+        sum_runs<4>([&](const float (&x)[V], int c) __attribute__((always_inline)) {
             uint32_t todo = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) todo |= x[i] >= open ? 1u << i : 0u;
@@ -906,18 +948,19 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
         __syncthreads();
     }
 
-    // How many labels of `each` reach the goal from front on
-    MFL_INLINE unsigned long long share_of(double goal, unsigned long long front, unsigned long long each) const
+    // How many labels of the mass `each` reach what is left
+    MFL_INLINE unsigned long long share_of(double left, double one, unsigned long long each) const
     {
-        unsigned long long n = (unsigned long long)fmax(1.0, __builtin_ceil((goal - (double)front) / (double)each));
-        while (n > 1 && (double)(front + (n - 1) * each) >= goal) --n;
-        while (n < (unsigned long long)C && (double)(front + n * each) < goal) ++n;
+        unsigned long long n = (unsigned long long)fmin(fmax(1.0, __builtin_ceil(left / ((double)each * one))), (double)C);
+        while (n > 1 && (double)((n - 1) * each) * one >= left) --n;
+        while (n < (unsigned long long)C && (double)(n * each) * one < left) ++n;
         return n;
     }
     // The rank key of the n-th label of one score, in label order (of the last one, if there are fewer)
     MFL_INLINE uint64_t nth_of_score(float score, unsigned long long n)
     {
-        sum_runs([&](const float (&x)[V], int c) __attribute__((always_inline)) {
+        // (two at a time: with four, the kernel's registers leave two waves a SIMD instead of three)
+        sum_runs<2>([&](const float (&x)[V], int c) __attribute__((always_inline)) {
             double found = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) found += x[i] == score && c + i < C ? 1.0 : 0.0;
@@ -978,7 +1021,7 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
                 const int b = bin_of(x);
                 if (by_count) atomicAdd(&sh.counts[b], 1u);
                 if (by_mass) {
-                    const uint64_t v = mass(x);
+                    const uint64_t v = mass(x, b);
                     if (v) atomicAdd(&sh.masses[b], (unsigned long long)v);
                 }
             });
@@ -988,64 +1031,55 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
 #pragma unroll 1
         for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {
             const bool count = stage == 0, final = stage == 1 || !by_mass;
-            // the bin it falls into, and what the bins in front of it hold
+            // the bin it falls into, and what the bins in front of it leave of the goal
             constexpr int each_bins = kBins / NT;
-            unsigned long long mine = 0, all;
-            for (int i = 0; i < each_bins; ++i) {
-                const int b = threadIdx.x * each_bins + i;
-                mine += count ? sh.counts[b] : sh.masses[b];
-            }
-            unsigned long long front = block_front<unsigned long long, NT>(mine, sh.upart, all);
-            // labels stay while what lies in front of them is below the goal
-            const double goal = count ? (double)f.top_k : f.top_p * (double)all;
-            if (threadIdx.x == 0) sh.listed = 0, sh.low_key = ~0ull, sh.bin = 0, sh.bin_front = 0;
-            __syncthreads();
-            if ((double)front < goal && (double)(front + mine) >= goal) {
-                int b = threadIdx.x * each_bins;
-                for (;; ++b) {
-                    const unsigned long long here = count ? sh.counts[b] : sh.masses[b];
-                    if ((double)(front + here) >= goal) break;
-                    front += here;
-                }
-                sh.bin = b;
-                sh.bin_front = front;
-            }
+            const auto held = [&](int b) __attribute__((always_inline)) { return count ? (double)sh.counts[b] : (double)sh.masses[b] * unit(b); };
+            if (threadIdx.x == 0) sh.reach.first = ~0u, sh.reach.last = 0, sh.listed = 0, sh.low_key = ~0ull;
             for (int i = threadIdx.x; i < kRuns; i += NT) sh.more[i] = 0;
-            __syncthreads();
-            bin = sh.bin;
-            front = sh.bin_front;
-            __syncthreads();
+            // (this thread's bins.  Made anew in each stage, or their steps are kept in registers throughout, which there are none for)
+            int own = threadIdx.x * each_bins;
+            asm volatile("" : "+v"(own));
+            double mine = 0, all;
+            for (int i = 0; i < each_bins; ++i) mine += held(own + i);
+            const double front = block_front<double, NT>(mine, sh.dpart, all);
+            // labels stay while what lies in front of them is below the goal
+            const double goal = count ? (double)f.top_k : f.top_p * all;
+            find_bin(each_bins, front, mine, goal, [&](int i) __attribute__((always_inline)) { return held(own + i); }, sh.reach);
+            bin = sh.reach.bin;
             sure = lowest_of(bin - 1);
             open = lowest_of(bin);
             sweep<true>(sure, open, cut, f.min_p);
             const int n = sh.listed;
+            const double one = count ? 1.0 : unit(bin);
+            // (rounded, but never more than the bin holds)
+            const double left = fmin(sh.reach.left, held(bin));
             if (n <= kBinList) {
                 for (int i = threadIdx.x; i < (n + 7) / 8 * 8; i += NT) {
                     if (i >= n) sh.key[i] = 0;
-                    sh.key_mass[i] = i >= n ? 0 : count ? 1 : mass(rank_score(sh.key[i]));
+                    sh.key_mass[i] = i >= n ? 0 : count ? 1 : mass(rank_score(sh.key[i]), bin);
                 }
                 __syncthreads();
                 for (int i = threadIdx.x; i < n; i += NT) {
                     const uint64_t key = sh.key[i];
                     const unsigned long long above = held_above(sh.key, sh.key_mass, n, key);
-                    // (a goal of next to nothing still keeps the first label)
-                    if (front + above == 0 || (double)(front + above) < goal) {
+                    // (a goal of nothing still keeps the first label)
+                    if (above == 0 || (double)above * one < left) {
                         atomicMin(&sh.low_key, key);
                         // (sums of integers: in any order)
                         if (final && weight(rank_score(key)) >= f.min_p)
-                            atomicAdd(&sh.more[rank_label(key) / (step * per)], (unsigned long long)mass(rank_score(key)));
+                            atomicAdd(&sh.more[rank_label(key) / (step * per)], (unsigned long long)mass(rank_score(key), bin));
                     }
                 }
                 __syncthreads();
                 cut = sh.low_key;
                 if (final) {
-                    for (int i = threadIdx.x; i < count_runs; i += NT) sh.runs[i] += __builtin_ldexp((double)sh.more[i], -bits);
+                    for (int i = threadIdx.x; i < count_runs; i += NT) sh.runs[i] += (double)sh.more[i] * unit(bin);
                     __syncthreads();
                     summed = true;
                 }
             } else {
-                // the largest key from which on at least `goal` is held, bit by bit where the bin's keys differ
-                if (threadIdx.x == 0) sh.low_key = ~0ull, sh.bin_front = 0;
+                // the largest key from which on the bin holds what is left of the goal, bit by bit where the bin's keys differ
+                if (threadIdx.x == 0) sh.low_key = ~0ull, sh.any_key = 0;
                 __syncthreads();
                 unsigned long long every = ~0ull, any = 0;
                 each([&](float x, int c) __attribute__((always_inline)) {
@@ -1055,13 +1089,13 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
                     any |= key;
                 });
                 atomicAnd(&sh.low_key, every);
-                atomicOr(&sh.bin_front, any);
+                atomicOr(&sh.any_key, any);
                 __syncthreads();
                 every = sh.low_key;
-                any = sh.bin_front;
+                any = sh.any_key;
                 uint64_t best = 0;
                 const bool one_score = every >> 32 == any >> 32;
-                if (one_score) best = nth_of_score(rank_score(any), share_of(goal, front, count ? 1 : mass(rank_score(any))));
+                if (one_score) best = nth_of_score(rank_score(any), share_of(left, one, count ? 1 : mass(rank_score(any), bin)));
 #pragma unroll 1
                 for (int b = one_score ? -1 : 63; b >= 0; --b) {
                     if (!(any >> b & 1)) continue;
@@ -1070,24 +1104,24 @@ template <typename T, int NT> struct BlockRow : Bins<4 * NT> {
                         best = at;
                         continue;
                     }
-                    unsigned long long held = 0;
+                    unsigned long long sum = 0;
                     each([&](float x, int c) __attribute__((always_inline)) {
-                        if (bin_of(x) == bin && rank_key(score_key(x), c) >= from) held += count ? 1 : mass(x);
+                        if (bin_of(x) == bin && rank_key(score_key(x), c) >= from) sum += count ? 1 : mass(x, bin);
                     });
-                    held = block_sum<unsigned long long, NT>(held, sh.upart);
-                    if (held && (double)(front + held) >= goal) best = at;
+                    sum = block_sum<unsigned long long, NT>(sum, sh.upart);
+                    if (sum && (double)sum * one >= left) best = at;
                 }
                 cut = best > cut ? best : cut;
             }
             if (!final) {
                 // what is left of the bin, and nothing behind it
-                unsigned long long left = 0;
+                unsigned long long kept = 0;
                 each([&](float x, int c) __attribute__((always_inline)) {
-                    if (bin_of(x) == bin && rank_key(score_key(x), c) >= cut) left += mass(x);
+                    if (bin_of(x) == bin && rank_key(score_key(x), c) >= cut) kept += mass(x, bin);
                 });
-                left = block_sum<unsigned long long, NT>(left, sh.upart);
+                kept = block_sum<unsigned long long, NT>(kept, sh.upart);
                 for (int i = threadIdx.x; i < kBins; i += NT)
-                    if (i >= bin) sh.masses[i] = i == bin ? left : 0;
+                    if (i >= bin) sh.masses[i] = i == bin ? kept : 0;
                 __syncthreads();
             }
         }
@@ -1417,8 +1451,8 @@ constexpr int kSplitParts = 512;
 constexpr unsigned kSplitRows = 128;
 struct SplitRow {
     unsigned long long masses[kSplitBins], keys[kBinList];
-    unsigned long long front;
-    double goal;
+    double left;                // of the goal, for the bin that the cut falls into
+    int bin;
     unsigned listed;
 };
 struct SplitSpace {
@@ -1469,8 +1503,9 @@ split_histogram_kernel(Rows in, Settings set, int parts, int size, SplitSpace ws
         const int c = begin + (u * kPlainThreads + (int)threadIdx.x) * V;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const uint64_t v = c + i < end ? bins.mass(x[u][i]) : 0;
-            if (v) atomicAdd(&masses[bins.bin_of(x[u][i])], (unsigned long long)v);
+            const int b = bins.bin_of(x[u][i]);
+            const uint64_t v = c + i < end ? bins.mass(x[u][i], b) : 0;
+            if (v) atomicAdd(&masses[b], (unsigned long long)v);
         }
     }
     __syncthreads();
@@ -1484,8 +1519,7 @@ split_sweep_kernel(Rows in, Settings set, int parts, int size, SplitSpace ws)
 {
     __shared__ float fpart[kPlainThreads / 64];
     __shared__ double dpart[kPlainThreads / 64];
-    __shared__ unsigned long long upart[kPlainThreads / 64], bin_front;
-    __shared__ int bin;
+    __shared__ Reach reach;
     constexpr int V = kVec<T>, U = kPlainVecs<T>, each_bins = kSplitBins / kPlainThreads;
     const unsigned r = blockIdx.x / parts, part = blockIdx.x - r * parts;
     const RowOf<T> row(in, r);
@@ -1501,28 +1535,18 @@ split_sweep_kernel(Rows in, Settings set, int parts, int size, SplitSpace ws)
     bins.set(m, f);
     float sure = -INFINITY, open = -INFINITY;
     if (f.top_p < 1) {
-        unsigned long long masses[each_bins], mine = 0, all;
-#pragma unroll
-        for (int i = 0; i < each_bins; ++i) mine += masses[i] = state.masses[threadIdx.x * each_bins + i];
-        unsigned long long front = block_front<unsigned long long, kPlainThreads>(mine, upart, all);
-        const double goal = f.top_p * (double)all;
-        if (threadIdx.x == 0) bin = 0, bin_front = 0;
-        __syncthreads();
-        if ((double)front < goal && (double)(front + mine) >= goal) {
-            int at = -1;
-            unsigned long long before = 0;
-#pragma unroll
-            for (int i = 0; i < each_bins; ++i) {
-                if (at < 0 && (double)(front + masses[i]) >= goal) at = i, before = front;
-                front += masses[i];
-            }
-            bin = threadIdx.x * each_bins + at;
-            bin_front = before;
-        }
-        __syncthreads();
-        sure = bins.lowest_of(bin - 1);
-        open = bins.lowest_of(bin);
-        if (part == 0 && threadIdx.x == 0) state.front = bin_front, state.goal = goal;
+        if (threadIdx.x == 0) reach.first = ~0u, reach.last = 0;
+        const auto held = [&](int i) {
+            const int b = threadIdx.x * each_bins + i;
+            return (double)state.masses[b] * bins.unit(b);
+        };
+        double mine = 0, all;
+        for (int i = 0; i < each_bins; ++i) mine += held(i);
+        const double front = block_front<double, kPlainThreads>(mine, dpart, all);
+        find_bin(each_bins, front, mine, f.top_p * all, held, reach);        // (the one thread reads its bins again)
+        sure = bins.lowest_of(reach.bin - 1);
+        open = bins.lowest_of(reach.bin);
+        if (part == 0 && threadIdx.x == 0) state.bin = reach.bin, state.left = reach.left;
     }
     double sum = 0;
 #pragma unroll
@@ -1582,20 +1606,22 @@ split_pick_kernel(Rows in, Settings set, int done, int parts, int size, SplitSpa
     }
     // the cut within the list
     uint64_t cut = 0;
+    Bins<kSplitBins> bins(in.C);
+    bins.set(m, f);
+    const int bin = ranked ? state.bin : 0;
     for (int i = threadIdx.x; i < parts; i += NT) more[i] = 0;
     if (ranked) {
         if (threadIdx.x == 0) sh.low_key = ~0ull;
         for (unsigned i = threadIdx.x; i < (n + 7) / 8 * 8; i += NT) {
             sh.key[i] = i < n ? state.keys[i] : 0;
-            sh.key_mass[i] = i < n ? row.mass(rank_score(sh.key[i])) : 0;
+            sh.key_mass[i] = i < n ? bins.mass(rank_score(sh.key[i]), bin) : 0;
         }
         __syncthreads();
-        const unsigned long long front = state.front;
-        const double goal = state.goal;
+        const double left = state.left, one = bins.unit(bin);
         for (unsigned i = threadIdx.x; i < n; i += NT) {
             const uint64_t key = sh.key[i];
             const unsigned long long above = held_above(sh.key, sh.key_mass, n, key);
-            if (front + above == 0 || (double)(front + above) < goal) {
+            if (above == 0 || (double)above * one < left) {
                 atomicMin(&sh.low_key, key);
                 if (row.weight(rank_score(key)) >= f.min_p) atomicAdd(&more[rank_label(key) / size], sh.key_mass[i]);
             }
@@ -1610,7 +1636,7 @@ split_pick_kernel(Rows in, Settings set, int done, int parts, int size, SplitSpa
         return w >= f.min_p ? w : 0.0;
     };
     double target = 0, total = 0;
-    const int part = find_entry(parts, [&](int i) { return part_of[i].sum + __builtin_ldexp((double)more[i], -row.bits); }, 0.0, uniform[r], target, total,
+    const int part = find_entry(parts, [&](int i) { return part_of[i].sum + (double)more[i] * bins.unit(bin); }, 0.0, uniform[r], target, total,
                                 false, sh.dpart, &first, &last, &before);
     const double front = before;
     __syncthreads();

@@ -249,7 +249,9 @@ inline bool temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }
 // Taylor polynomial of 2^f to f^11 (the next term is 2^-47).  The largest score weighs exactly 1.
 struct Weight {
     double m, a;                // a = log2(e) / temperature
-    __device__ double operator()(float x) const
+    __device__ double operator()(float x) const { return scaled(x, 0); }
+    // ... times 2^by
+    __device__ double scaled(float x, int by) const
     {
         const double y = fmax(((double)x - m) * a, -1100.0);     // (2^-1100 is 0; -inf would leave f undefined)
         const double n = __builtin_rint(y), f = y - n;
@@ -265,7 +267,7 @@ struct Weight {
         p = fma(p, f, 2.4022650695910071e-01);
         p = fma(p, f, 6.9314718055994531e-01);
         p = fma(p, f, 1.0);
-        return __builtin_ldexp(p, (int)n);
+        return __builtin_ldexp(p, (int)n + by);
     }
 };
 

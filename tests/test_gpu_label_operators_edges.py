@@ -113,3 +113,40 @@ def test_rest_of_rows_that_are_no_numbers(C, k, S):
     x[4, : k + 1], x[4, k + 1] = INF, -INF                 # infinities alone: an infinite rest
     for y in (x, x.reshape(2, 3, C).movedim(2, 1)):
         G.check_top(S, y, k, 1.0)
+
+
+# ------------------------------------------------------------------ drawn labels
+
+def long_draw(z, us, top_k, top_p):
+    """R.sample for many draws of one row, in 80-bit arithmetic: next to a largest weight of 1 the sum of 10^5 weights of
+    2^-44 is lost in the steps of 64 bits."""
+    z = np.asarray(z, np.longdouble)
+    w = np.exp(z - z.max())
+    order = R.order_of(z)[: top_k or z.size]
+    front = np.concatenate([[np.longdouble(0)], np.cumsum(w[order])])
+    n = max(1, int((front[:-1] < np.longdouble(top_p) * front[-1]).sum())) if top_p < 1 else order.size
+    keep = np.sort(order[:n])
+    run = np.cumsum(w[keep])
+    at = [min(int(np.searchsorted(run, np.longdouble(u) * run[-1], side="right")), n - 1) for u in us]
+    return keep[at], np.array([np.log(w[keep[i]] / run[-1]) for i in at], np.float64), n
+
+
+@pytest.mark.parametrize("rows,C,low,high,top_k", [(5, 1 << 20, 30.2, 30.2, 0), (5, 1 << 19, 28.5, 31.9, 0), (130, 1 << 19, 28.5, 31.9, 0),
+                                                   (5, 1 << 19, 28.5, 36.0, 1 << 18), (5, 1 << 20, 30.2, 30.2, 1 << 19)])
+def test_a_cut_deep_in_the_tail(rows, C, low, high, top_k, S):
+    """One peak and a tail of labels 2^-41 to 2^-52 of it, which top_p cuts in the middle: every label of the tail keeps the
+    mass it has.  The draws fall into the tail, whose labels stand in front of the peak."""
+    gen = np.random.default_rng(7)
+    z = -gen.permutation(np.linspace(low, high, C)).astype(np.float32)
+    z[C - 1] = 0
+    kept = np.sort(np.exp(z.astype(np.longdouble)))[::-1][: top_k or C]
+    mass = float(kept[1:].sum())
+    top_p = 1.0 - 0.5 * mass
+    us = np.float32(mass * np.linspace(0.0, 0.45, 5)).tolist()
+    want, logprob, n = long_draw(z, us, top_k, top_p)
+    assert 2048 < n < C - 2048 and len(set(want.tolist())) == 5
+    x = torch.from_numpy(z).cuda().expand(rows, C).contiguous()
+    u = torch.tensor(us, dtype=torch.float32, device="cuda").repeat(rows // 5)
+    got, lp = S.ops.sample_labels(x, u, top_k=top_k, top_p=top_p, want_logprob=True)
+    assert got.cpu().numpy().tolist() == want.tolist() * (rows // 5)
+    assert (np.abs(lp.cpu().numpy()[:5] - logprob) <= 2.0 ** -24 * np.abs(logprob) + 1e-9).all()
