@@ -150,3 +150,22 @@ def test_a_cut_deep_in_the_tail(rows, C, low, high, top_k, S):
     got, lp = S.ops.sample_labels(x, u, top_k=top_k, top_p=top_p, want_logprob=True)
     assert got.cpu().numpy().tolist() == want.tolist() * (rows // 5)
     assert (np.abs(lp.cpu().numpy()[:5] - logprob) <= 2.0 ** -24 * np.abs(logprob) + 1e-9).all()
+
+
+@pytest.mark.parametrize("shape,scale", [((3, 4096), 0.01), ((140, 9000), 0.004), ((4, 60000), 0.05), ((2, 200000), 0.1)])
+def test_cuts_within_a_bin_of_many_different_scores(shape, scale, S):
+    """Rows so flat that the part of the row the cut falls into holds more labels than its list, of different scores."""
+    x = G.scores_of(shape, torch.float32, 281, scale)
+    if shape[0] > 100:
+        x[3:] = x[:1]                                      # (the restatement walks three rows; the others repeat the first)
+    u = torch.rand(shape[0], generator=G.gen(282), device="cuda")
+    if shape[0] > 100:
+        u[3:] = u[0]
+    C = shape[1]
+    for kw in (dict(top_p=0.8), dict(top_p=0.5, min_p=0.9), dict(top_k=C // 3), dict(top_k=C // 2, top_p=0.7)):
+        labels, logprob = S.ops.sample_labels(x, u, want_logprob=True, **kw)
+        for i in range(min(3, shape[0])):
+            want, lp = R.sample(x[i].cpu().numpy(), float(u[i]), **kw)
+            assert int(labels[i]) == want and abs(float(logprob[i]) - lp) <= 2.0 ** -24 * abs(lp) + 1e-12, (i, kw)
+        if shape[0] > 100:
+            assert (labels[3:] == labels[0]).all()
