@@ -770,7 +770,8 @@ template <int BINS> struct Bins {
         scale = (float)fmin(f.inv_t * (BINS / kUnits), 1e30);
         weight = {m, f.inv_t * kLog2eD};
     }
-    MFL_INLINE int bin_of(float x) const { return min((int)((m - x) * scale), BINS - 1); }
+    // (the smaller one before the conversion: -inf has no integer)
+    MFL_INLINE int bin_of(float x) const { return (int)fminf((m - x) * scale, (float)(BINS - 1)); }
     MFL_INLINE uint64_t mass(float x, int bin) const
     {
         // 2^52 + an integer below 2^52: the low bits of the sum are that integer
