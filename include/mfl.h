@@ -344,7 +344,9 @@ int mfl_resize_labels(const unsigned char *src, int H0, int W0, const int *yin, 
  * Operators on rows of scores.  A row is one distribution over C labels; element (n, c, s) of N x C x S scores lies at
  * scores + n * stride_n + c * stride_c + s * stride_s (elements; not negative), so [B][C][H][W] maps (S = H*W), [N][C]
  * matrices (S = 1), channels-last maps and slices are read where they are.  dtype: MFL_F32, MFL_BF16 or MFL_F16.
- * N * S < 2^31 and C <= 2^30 (MFL_ERR_TOO_LARGE); offsets are 64-bit.  b = score / temperature throughout.
+ * N * S < 2^31 and C <= 2^30; offsets are 64-bit.  Rows of many labels take a wave or workgroups each, of a launch's 2^32
+ * threads: N * S < 2^24 for them (drawing at C > 4096: 2^24 / ceil(C / 8192) without filters, 2^22 under top_p or a top_k
+ * above 128).  Beyond that: MFL_ERR_TOO_LARGE.  b = score / temperature throughout.
  * Results do not depend on the launch or on timing: no floating-point atomics.
  *
  * mfl_top_labels: the k largest scores of every row, descending, the lower label first among equals (a NaN counts as

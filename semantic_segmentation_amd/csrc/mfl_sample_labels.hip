@@ -1659,6 +1659,8 @@ int list_length(const Settings &set)
     return set.top_k >= 1 && set.top_k <= MFL_MAX_TOP_LABELS ? set.top_k : 0;
 }
 
+constexpr int kShortRow = 4096;             // a workgroup of 256 up to here, of 1024 above
+
 enum Way { LONE, LANES, LIST_LANES, ANY_LANES, PLAIN, WAVES, SPLIT, BLOCKS };
 struct Plan {
     Way way;
@@ -1698,11 +1700,11 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
 {
     const Plan plan = plan_of(in, set);
     const int k = plan.k;
-    const unsigned threads_a_row = plan.way == PLAIN  ? kPlainThreads * plain_parts(in.rows, in.C)
-                                   : plan.way < PLAIN ? 1
-                                   : plan.way == WAVES && !plan.two && row_per_wave(in.rows, in.C) ? 64
-                                   : plan.way == WAVES && !plan.two ? kWaveTopThreads * top_parts(in.rows, in.C)
-                                                                    : 1024;
+    // the threads that a row takes in the largest of the launches
+    unsigned threads_a_row = 1;
+    if (plan.way == WAVES) threads_a_row = row_per_wave(in.rows, in.C) ? 64 : kWaveTopThreads * top_parts(in.rows, in.C);
+    if (plan.way == PLAIN || plan.split) threads_a_row = max(threads_a_row, (unsigned)(kPlainThreads * plain_parts(in.rows, in.C)));
+    else if (plan.way == BLOCKS || plan.two) threads_a_row = max(threads_a_row, in.C <= kShortRow ? 256u : 1024u);
     if (!launchable(in.rows, threads_a_row)) return MFL_ERR_TOO_LARGE;
     const dim3 grid((in.rows + kLaneThreads - 1) / kLaneThreads), block(kLaneThreads);
 #define MFL_LANES(...) hipLaunchKernelGGL(__VA_ARGS__, grid, block, 0, st, in, set, uniform, out)
@@ -1767,7 +1769,7 @@ int run(const Rows &in, const Settings &set, const float *uniform, const Out &ou
             hipLaunchKernelGGL(split_pick_kernel<T>, one, threads, 0, st, in, set, k, parts, size, ws, uniform, out);
             break;
         }
-        if (in.C <= 4096) hipLaunchKernelGGL((sample_blocks_kernel<T, 256>), dim3(in.rows), dim3(256), 0, st, in, set, k, uniform, out);
+        if (in.C <= kShortRow) hipLaunchKernelGGL((sample_blocks_kernel<T, 256>), dim3(in.rows), dim3(256), 0, st, in, set, k, uniform, out);
         else hipLaunchKernelGGL((sample_blocks_kernel<T, 1024>), dim3(in.rows), dim3(1024), 0, st, in, set, k, uniform, out);
     }
     return (int)hipGetLastError();

@@ -215,7 +215,9 @@ _F32, _I32, _FLAGS = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
 def top_labels(scores: torch.Tensor, k: int, temperature: float = 1.0):
     """The k largest scores of every row of [N, C] or [N, C, ...] scores, descending, the lower label first among equals:
     (values [N, k, ...] of the scores' type, labels [N, k, ...] int32, rest [N, ...] float32), with rest = log sum
-    exp(score / temperature) over all other labels (-inf if there are none).  The record distillation_forward reads."""
+    exp(score / temperature) over all other labels (-inf if there are none).  The record distillation_forward reads.
+    Up to 2^31 rows, of many labels (each a wave's or a workgroup's work) 2^24, as in the other operators on rows of scores;
+    more raise MflError."""
     v, args = _score_rows(scores)
     k = int(k)
     if not 1 <= k <= min(args[3], _lib.MAX_TOP_LABELS):

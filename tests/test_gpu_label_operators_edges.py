@@ -169,3 +169,14 @@ def test_cuts_within_a_bin_of_many_different_scores(shape, scale, S):
             assert int(labels[i]) == want and abs(float(logprob[i]) - lp) <= 2.0 ** -24 * abs(lp) + 1e-12, (i, kw)
         if shape[0] > 100:
             assert (labels[3:] == labels[0]).all()
+
+
+def test_drawing_for_very_many_rows_of_a_few_hundred_labels(S):
+    """2^22 and more rows that a workgroup each draws for (all of them one row of memory, seen with stride 0)."""
+    n, C = (1 << 22) + 8, 256
+    z = G.scores_of((1, C), torch.bfloat16, 291, 2.0)
+    u = torch.rand(n, generator=G.gen(292), device="cuda")
+    labels = S.ops.sample_labels(z.expand(n, C), u, top_p=0.9, dtype=torch.int32)
+    for i in (0, 1, n // 2, n - 9, n - 8, n - 1):
+        assert int(labels[i]) == R.sample(z[0].float().cpu().numpy(), float(u[i]), top_p=0.9)[0]
+    assert torch.equal(labels[-8:], S.ops.sample_labels(z.expand(8, C), u[-8:], top_p=0.9, dtype=torch.int32))
