@@ -372,6 +372,7 @@ int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long
  *   values: [N][k][S] of values_dtype   labels: [N][k][S] int32   rest: [N][S] float or NULL (entries renormalised)
  *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [5][N][S] floats, from forward to backward
  *   grad_loss: [N][S]   d_scores: the scores' type, with strides of its own, overwritten
+ *   1 <= k <= MFL_MAX_TOP_LABELS, 1e-18 <= temperature <= 1e18
  */
 size_t mfl_distillation_workspace_bytes(int N, int C, int S, int dtype, int k);
 int mfl_distillation_forward(const void *scores, int dtype, int N, int C, int S, long long stride_n, long long stride_c,

@@ -732,7 +732,8 @@ int run_backward(const Rows &in, const Teacher &t, const float *stats, const flo
 int make_teacher(Teacher &t, const void *values, int dtype, const int *labels, const float *rest, const unsigned char *valid, int k,
                  double temperature)
 {
-    if (!values || !labels || k < 1 || k > MFL_MAX_TOP_LABELS || !temperature_ok(temperature)) return MFL_ERR_INVALID_ARGUMENT;
+    // (the loss is T^2 times a sum: an ordinary fp32 number as well, or a loss of 0 becomes a NaN)
+    if (!values || !labels || k < 1 || k > MFL_MAX_TOP_LABELS || !(temperature >= 1e-18 && temperature <= 1e18)) return MFL_ERR_INVALID_ARGUMENT;
     if (dtype != MFL_F32 && dtype != MFL_BF16 && dtype != MFL_F16) return MFL_ERR_INVALID_ARGUMENT;
     t = {values, dtype, labels, rest, valid, k, (float)(kLog2eD / temperature), (float)(1.0 / temperature), (float)temperature};
     return MFL_OK;

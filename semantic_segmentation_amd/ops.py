@@ -273,9 +273,9 @@ def _distillation_backward(scores, v, args, record, stats, grad_loss, temperatur
 
 def distillation_forward(scores, top_scores, top_labels, rest=None, temperature: float = 1.0, valid=None):
     """Loss of every row of [N, C, ...] scores against a teacher's record (top_labels of the teacher's scores at the same
-    temperature): T^2 KL(teacher || softmax(scores / T)) over the record's labels and, with `rest`, everything else as one
-    more outcome; without it the record is renormalised.  Labels outside [0, C) are passed over; rows with valid = False or
-    without teacher mass have loss 0.  Returns (loss [N, ...] float32, stats for distillation_backward)."""
+    temperature, T between 1e-18 and 1e18): T^2 KL(teacher || softmax(scores / T)) over the record's labels and, with `rest`,
+    everything else as one more outcome; without it the record is renormalised.  Labels outside [0, C) are passed over; rows
+    with valid = False or without teacher mass have loss 0.  Returns (loss [N, ...] float32, stats for distillation_backward)."""
     v, args = _score_rows(scores)
     _, record, rows = _record(scores, top_scores, top_labels, rest, valid)
     return _distillation_forward(scores, v, args, record, rows, temperature)

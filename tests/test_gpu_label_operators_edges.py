@@ -98,6 +98,23 @@ def test_distillation_of_records_that_are_no_numbers(C, planes, S):
     G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), lay_rows(rest, planes), 1.5)
 
 
+@pytest.mark.parametrize("C", [21, 600])
+def test_distillation_temperatures(C, S):
+    """T^2 has to be an ordinary fp32 number; at the ends of the range results stay finite."""
+    x = G.scores_of((3, C), torch.float32, 231)
+    values, labels, rest = G.record_of(x, 3, 1.0, 232)
+    for t in (1e-30, 1e-19, 1e19, 1e30):
+        with pytest.raises(ValueError):
+            S.ops.distillation_forward(x, values, labels, rest, t)
+        loss = torch.ones(3, device="cuda")
+        with pytest.raises(ValueError):
+            S.ops.distillation_backward(x, values, labels, S.ops.distillation_forward(x, values, labels, rest)[1], loss, rest, t)
+    for t in (1e-18, 1e18):
+        loss, stats = S.ops.distillation_forward(x, values, labels, None, t)
+        assert torch.isfinite(loss).all()
+        assert torch.isfinite(S.ops.distillation_backward(x, values, labels, stats, torch.ones_like(loss), None, t)).all()
+
+
 # ------------------------------------------------------------------ top labels
 
 @pytest.mark.parametrize("C,k", [(40, 3), (300, 3), (700, 20), (9000, 3), (9000, 100)])
