@@ -64,6 +64,8 @@ extern "C" {
 #define MFL_F16 2
 /* most labels a record of top labels holds */
 #define MFL_MAX_TOP_LABELS 128
+/* up to this many labels mfl_distillation_backward needs no statistics of mfl_distillation_forward */
+#define MFL_DISTILLATION_LONE_LABELS 24
 
 typedef void *mfl_stream_t;
 
@@ -370,7 +372,8 @@ int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long
  * twice counts as two entries.  Rows with valid = 0, without any teacher mass or whose scores are all -inf have loss 0
  * and gradient 0, whatever the other tensors hold there.
  *   values: [N][k][S] of values_dtype   labels: [N][k][S] int32   rest: [N][S] float or NULL (entries renormalised)
- *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [5][N][S] floats, from forward to backward
+ *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [5][N][S] floats, from forward to backward (neither written nor
+ *   read for C <= MFL_DISTILLATION_LONE_LABELS, where any address but NULL will do)
  *   grad_loss: [N][S]   d_scores: the scores' type, with strides of its own, overwritten
  *   1 <= k <= MFL_MAX_TOP_LABELS, 1e-18 <= temperature <= 1e18
  */

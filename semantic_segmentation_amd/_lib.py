@@ -25,6 +25,7 @@ _c_ll, _c_double = ctypes.c_longlong, ctypes.c_double
 _SCORES = [_c_void] + [_c_int] * 4 + [_c_ll] * 3        # scores, dtype, N, C, S and three strides
 SCORE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # MFL_F32, MFL_BF16, MFL_F16
 MAX_TOP_LABELS = 128
+DISTILLATION_LONE_LABELS = 24
 
 # name -> (restype, argtypes); mirrors include/mfl.h one to one
 SIGNATURES = {

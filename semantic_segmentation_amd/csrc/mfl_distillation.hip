@@ -15,7 +15,9 @@
 // Z_O is summed directly over O, never as a difference: where the record holds nearly all the mass, Z - (record) would
 // leave nothing but rounding.  Softmax statistics are fp32 as (m, log s) with m the row's largest score, which is exact:
 // differences b_i - Z then lose nothing to the size of the scores.
-//   stats[0] = m,  stats[1] = Z - m / T,  stats[2] = Z_O - Z (0 without rest)
+//   stats[0] = m,  stats[1] = Z - m / T,  stats[2] = m_O, the largest score in O,  stats[3] = Z_O - m_O / T,  stats[4] = Z_O - Z
+// without anything in O: m_O and Z_O - Z are -inf, Z_O - m_O / T is 0; a row without loss: the same of m and Z - m / T too; a
+// row with a NaN score: all NaN.  Up to kLoneBlock labels nothing is kept, the backward pass finds them anew.
 //
 // Both passes are bound by memory: the forward pass reads the scores, the backward pass reads them again and writes the
 // gradient.  Measured on MI355X, forward / backward: 8 x 21 x 512 x 512 fp32, k = 4 with rest 58 / 96 us (4.5 TB/s each);
@@ -154,7 +156,7 @@ __device__ inline float slope(const Slope &s, float x, float taken, float c2)
 // CB >= C the scores do, and the backward pass then finds the softmax statistics by itself instead of reading them back
 // (16 bytes of 200 a pixel at 21 labels).
 
-constexpr int kLoneBlock = 24;          // up to this many labels a lane's scores stay in registers
+constexpr int kLoneBlock = MFL_DISTILLATION_LONE_LABELS;        // up to this many labels a lane's scores stay in registers
 
 // Entries j0 .. j0 + KB of a row's record; x: the student's scores of their labels
 template <typename T, int KB> struct Block {

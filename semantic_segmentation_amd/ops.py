@@ -250,13 +250,19 @@ def _record(scores, top_scores, top_labels, rest, valid):
                                                    _address(rest), _address(valid), k), rows
 
 
+def _stats_shape(scores, rows):
+    """Statistics a row that forward keeps for backward: none of few labels, which backward finds anew."""
+    return ((0 if scores.shape[1] <= _lib.DISTILLATION_LONE_LABELS else 5),) + rows
+
+
 def _distillation_forward(scores, v, args, record, rows, temperature):
     loss = torch.empty(rows, dtype=torch.float32, device=scores.device)
-    stats = torch.empty((5,) + rows, dtype=torch.float32, device=scores.device)
+    stats = torch.empty(_stats_shape(scores, rows), dtype=torch.float32, device=scores.device)
     n = lib.mfl_distillation_workspace_bytes(*args[2:5], args[1], record[5])
     ws = torch.empty(n, dtype=torch.uint8, device=scores.device) if n else None
+    # (where there are none, an address that is not NULL)
     _lib.call_scores(lib.mfl_distillation_forward, "mfl_distillation_forward", v, *args, *record, float(temperature), loss.data_ptr(),
-                     stats.data_ptr(), _address(ws), n)
+                     stats.data_ptr() or loss.data_ptr(), _address(ws), n)
     return loss, stats
 
 
@@ -266,8 +272,8 @@ def _distillation_backward(scores, v, args, record, stats, grad_loss, temperatur
     if out[0] != grad.data_ptr():                          # (a layout without one common stride)
         grad = torch.empty_like(scores, memory_format=torch.contiguous_format, requires_grad=False)
         g, out = _score_rows(grad, "the gradient")
-    _lib.call_scores(lib.mfl_distillation_backward, "mfl_distillation_backward", v, *args, *record, float(temperature), stats.data_ptr(),
-                     grad_loss.data_ptr(), out[0], *out[5:])
+    _lib.call_scores(lib.mfl_distillation_backward, "mfl_distillation_backward", v, *args, *record, float(temperature),
+                     stats.data_ptr() or grad_loss.data_ptr(), grad_loss.data_ptr(), out[0], *out[5:])
     return grad
 
 
@@ -275,7 +281,8 @@ def distillation_forward(scores, top_scores, top_labels, rest=None, temperature:
     """Loss of every row of [N, C, ...] scores against a teacher's record (top_labels of the teacher's scores at the same
     temperature, T between 1e-18 and 1e18): T^2 KL(teacher || softmax(scores / T)) over the record's labels and, with `rest`,
     everything else as one more outcome; without it the record is renormalised.  Labels outside [0, C) are passed over; rows
-    with valid = False or without teacher mass have loss 0.  Returns (loss [N, ...] float32, stats for distillation_backward)."""
+    with valid = False or without teacher mass have loss 0.  Returns (loss [N, ...] float32, stats for distillation_backward,
+    [5, N, ...] float32 and empty, [0, N, ...], up to 24 labels)."""
     v, args = _score_rows(scores)
     _, record, rows = _record(scores, top_scores, top_labels, rest, valid)
     return _distillation_forward(scores, v, args, record, rows, temperature)
@@ -286,7 +293,7 @@ def distillation_backward(scores, top_scores, top_labels, stats, grad_loss, rest
     the other arguments as there, stats as it returned them."""
     v, args = _score_rows(scores)
     _, record, rows = _record(scores, top_scores, top_labels, rest, valid)
-    stats = _beside(scores, stats, "stats", _F32, (5,) + rows)
+    stats = _beside(scores, stats, "stats", _F32, _stats_shape(scores, rows))
     grad_loss = _beside(scores, grad_loss, "grad_loss", _F32, rows)
     return _distillation_backward(scores, v, args, record, stats, grad_loss, temperature)
 

@@ -115,6 +115,23 @@ def test_distillation_temperatures(C, S):
         assert torch.isfinite(S.ops.distillation_backward(x, values, labels, stats, torch.ones_like(loss), None, t)).all()
 
 
+def test_distillation_statistics(S):
+    """What forward hands to backward: five numbers a row, written in full, or nothing where backward needs nothing."""
+    for C, n in [(2, 0), (24, 0), (25, 5), (300, 5)]:
+        x = G.scores_of((2, C, 7, 9), torch.float32, 241)
+        values, labels, rest = G.record_of(x, 2, 1.0, 242)
+        loss, stats = S.ops.distillation_forward(x, values, labels, rest)
+        assert tuple(stats.shape) == (n, 2, 7, 9) and torch.isfinite(stats).all()
+        if n:
+            z = torch.logsumexp(x.double(), 1) - x.max(1).values.double()
+            assert torch.equal(stats[0], x.max(1).values) and float((stats[1].double() - z).abs().max()) <= G.CHAIN(C) * 2.0 ** -24 + 2.0 ** -20
+        leaf = x.clone().requires_grad_(True)
+        grad, = torch.autograd.grad(S.training.distillation_loss(leaf, values, labels, rest).sum(), leaf)
+        assert torch.equal(grad, S.ops.distillation_backward(x, values, labels, stats, torch.ones_like(loss), rest))
+        with pytest.raises(RuntimeError):
+            S.ops.distillation_backward(x, values, labels, torch.zeros((5 - n, 2, 7, 9), device="cuda"), torch.ones_like(loss), rest)
+
+
 # ------------------------------------------------------------------ top labels
 
 @pytest.mark.parametrize("C,k", [(40, 3), (300, 3), (700, 20), (9000, 3), (9000, 100)])
