@@ -81,11 +81,13 @@ def per_image_distillation(scores: torch.Tensor, top_scores: torch.Tensor, top_l
                            rest: Optional[torch.Tensor] = None, temperature: float = 1.0,
                            valid: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Mean over the batch of every image's mean distillation loss over its valid pixels: per_image_nll with the teacher's
-    distribution as the target.  An image without a valid pixel contributes 0."""
-    losses = distillation_loss(scores, top_scores, top_labels, rest, temperature, valid).flatten(1)
+    distribution as the target.  An image without a valid pixel contributes 0.  (A row of [N, C] scores is an image of one
+    pixel.)"""
+    losses = distillation_loss(scores, top_scores, top_labels, rest, temperature, valid)
+    losses = losses.reshape(losses.shape[0], -1)
     if valid is None:
         return losses.mean(1).mean()
-    return (losses.sum(1) / (valid != 0).flatten(1).sum(1).clamp(min=1)).mean()
+    return (losses.sum(1) / (valid != 0).reshape(losses.shape).sum(1).clamp(min=1)).mean()
 
 
 def fit(model: nn.Module, optimizer: torch.optim.Optimizer,

@@ -132,6 +132,20 @@ def test_distillation_statistics(S):
             S.ops.distillation_backward(x, values, labels, torch.zeros((5 - n, 2, 7, 9), device="cuda"), torch.ones_like(loss), rest)
 
 
+def test_per_image_distillation_of_a_matrix(S):
+    """[N, C] scores: every row an image of one pixel."""
+    x = G.scores_of((6, 40), torch.float32, 251)
+    values, labels, rest = G.record_of(x, 4, 1.0, 252)
+    valid = torch.tensor([1, 0, 1, 1, 0, 1], dtype=torch.bool, device="cuda")
+    as_map = lambda a: a.unsqueeze(-1).unsqueeze(-1)
+    for v in (valid, None):
+        got = S.training.per_image_distillation(x, values, labels, rest, 1.0, v)
+        want = S.training.per_image_distillation(as_map(x), as_map(values), as_map(labels), as_map(rest), 1.0, None if v is None else as_map(v))
+        rows = S.training.distillation_loss(x, values, labels, rest, 1.0, v).double()
+        assert got.shape == () and abs(float(got) - float(rows.mean())) <= 8 * 2.0 ** -24 * float(rows.mean())
+        assert abs(float(got) - float(want)) <= 16 * 2.0 ** -24 * float(rows.mean())
+
+
 # ------------------------------------------------------------------ top labels
 
 @pytest.mark.parametrize("C,k", [(40, 3), (300, 3), (700, 20), (9000, 3), (9000, 100)])
