@@ -146,6 +146,41 @@ def test_per_image_distillation_of_a_matrix(S):
         assert abs(float(got) - float(want)) <= 16 * 2.0 ** -24 * float(rows.mean())
 
 
+@pytest.mark.parametrize("by_rows", [True, False])
+def test_distillation_gradient_past_32_bits(by_rows, S):
+    """2^31 + scores whose last rows lie past 32-bit element offsets, against a teacher that differs from the student there:
+    a gradient far from zero."""
+    if by_rows:
+        n, c = 33000, 65600
+        x = torch.zeros(n, c, dtype=torch.bfloat16, device="cuda")
+        rows = G.scores_of((3, c), torch.bfloat16, 261)
+        x[n - 3:] = rows
+        tail = lambda t: t[n - 3:]
+    else:
+        c, h, w = 33, 8192, 8192
+        x = torch.zeros(1, c, h, w, dtype=torch.bfloat16, device="cuda")
+        rows = G.scores_of((3, c), torch.bfloat16, 262)
+        x[0, :, h - 1, w - 3:] = rows.t()
+        tail = lambda t: t[0, ..., h - 1, w - 3:].t() if t.dim() == 4 else t[0, h - 1, w - 3:]
+    k = 3
+    values, labels, rest = G.record_of(rows, k, 1.0, 263)
+    outer = (x.shape[0],) + tuple(x.shape[2:])
+    full = lambda shape, dtype, value, part: (lambda t: (tail(t).copy_(part), t)[1])(torch.full(shape, value, dtype=dtype, device="cuda"))
+    wide = (x.shape[0], k) + tuple(x.shape[2:])
+    values_all, labels_all, rest_all = full(wide, values.dtype, 1.0, values), full(wide, torch.int32, 0, labels), full(outer, torch.float32, 0.5, rest)
+    loss, stats = S.ops.distillation_forward(x, values_all, labels_all, rest_all)
+    # (so that memory of an earlier gradient does not pass for this one)
+    torch.full_like(x, 7.0)
+    grad = S.ops.distillation_backward(x, values_all, labels_all, stats, torch.ones_like(loss), rest_all)
+    got_l, got_g, half = tail(loss).cpu().numpy(), tail(grad).float().cpu().numpy(), 2.0 ** -8
+    unit = G.CHAIN(c) * 2.0 ** -23 + 2.0 ** -21
+    for i in range(3):
+        wl, wg, (bl, bg) = R.distill(rows[i].double().cpu().numpy(), values[i].float().cpu().numpy(), labels[i].cpu().numpy(), float(rest[i]), 1.0)
+        assert wl > 0.01 and abs(got_l[i] - wl) <= unit * bl
+        assert np.abs(wg).max() > 0.01
+        assert (np.abs(got_g[i] - wg) <= unit * bg * (1 + half) + half * np.abs(wg) + 2.0 ** -125).all()
+
+
 # ------------------------------------------------------------------ top labels
 
 @pytest.mark.parametrize("C,k", [(40, 3), (300, 3), (700, 20), (9000, 3), (9000, 100)])
