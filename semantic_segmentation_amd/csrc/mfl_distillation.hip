@@ -67,14 +67,20 @@ __device__ inline Target target_of(const Teacher &t, Excess sum, bool named, flo
 }
 __device__ inline float log_share(const Teacher &t, const Target &g, float value) { return (value - g.m) * t.inv_t - g.l; }
 
-// p (log p - log q); nothing where p is 0
-__device__ inline float share_term(float p, float log_p, float log_q) { return p == 0.f ? 0.f : p * (log_p - log_q); }
-// ... of an entry: log p - log q = ((t - m_p) - (score - m_q)) / T - log((1 + s_p) / (1 + s_q)), in this order, since close
-// to the teacher the two logarithms agree in most of their digits
+// p T d; nothing where p is 0.  (A share that fp32 does not hold still counts next to a difference near the largest number.)
+__device__ inline float share_term(float log_p, float t, float d)
+{
+    const float e = log_p * kLog2e;
+    const bool tiny = e < -100.f;
+    const float p = __builtin_amdgcn_exp2f(tiny ? e + 60.f : e);
+    return p == 0.f ? 0.f : p * t * (tiny ? d * 0x1p-60f : d);
+}
+// T^2 p (log p - log q) of an entry.  log p - log q = ((t - m_p) - (score - m_q)) / T -
+// log((1 + s_p) / (1 + s_q)), in this order, since close to the teacher the two logarithms agree in most of their digits, and
+// times T, since a score of the type's lowest number over T may be no fp32 number where T times it is one
 __device__ inline float entry_term(const Teacher &t, const Target &g, float log_sums, float m, float value, float x)
 {
-    const float p = __builtin_amdgcn_exp2f(log_share(t, g, value) * kLog2e);
-    return p == 0.f ? 0.f : p * fmaf((value - g.m) - (x - m), t.inv_t, -log_sums);
+    return share_term(log_share(t, g, value), t.t, fmaf(-log_sums, t.t, (value - g.m) - (x - m)));
 }
 
 struct Stats {
@@ -82,6 +88,12 @@ struct Stats {
     float s;                            // z = log(1 + s); not kept
 };
 constexpr Stats kNoStats = {-INFINITY, 0.f, -INFINITY, 0.f, -INFINITY, 0.f};
+// ... of the rest (without it log p_rest is -inf)
+__device__ inline float rest_term(const Teacher &t, const Target &g, const Stats &a)
+{
+    const float d = a.log_q_rest == -INFINITY && a.mo != -INFINITY ? fmaf(g.log_p_rest - (a.zo - a.z), t.t, a.m - a.mo) : (g.log_p_rest - a.log_q_rest) * t.t;
+    return share_term(g.log_p_rest, t.t, d);
+}
 // log((1 + s_p) / (1 + s_q))
 __device__ inline float log_sums(const Target &g, const Stats &a)
 {
@@ -317,14 +329,14 @@ forward_lanes_kernel(Rows in, Teacher t, float *__restrict__ loss, float *__rest
     const Stats a = stats_of(top, out, t);
     if (!flags.valid(t) || !g.any || a.m == -INFINITY) return put(loss, LONE ? nullptr : stats, in.rows, r, 0.f, kNoStats);
     const float dl = log_sums(g, a);
-    float sum = t.rest ? share_term(g.p_rest, g.log_p_rest, a.log_q_rest) : 0.f;
+    float sum = rest_term(t, g, a);
     record.each([&](const Block<T, KB> &b) {
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
             sum += b.label[j] >= 0 ? entry_term(t, g, dl, a.m, b.value[j], b.x[j]) : 0.f;
         }
     });
-    put(loss, LONE ? nullptr : stats, in.rows, r, t.t * t.t * sum, a);
+    put(loss, LONE ? nullptr : stats, in.rows, r, sum, a);
 }
 
 // What the record takes from each label of a block lies in LDS, one column per lane (-1: not named).
@@ -559,8 +571,8 @@ finish_rows_kernel(Rows in, Teacher t, int parts, const LogSum *__restrict__ sum
     for (int h = 0; h < 2; ++h) sum += e.in[h] ? entry_term(t, g, dl, a.m, e.value[h], x[h]) : 0.f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (t.rest) sum += share_term(g.p_rest, g.log_p_rest, a.log_q_rest);
-    if (lane == 0) put(loss, stats, in.rows, r, t.t * t.t * sum, a);
+    sum += rest_term(t, g, a);
+    if (lane == 0) put(loss, stats, in.rows, r, sum, a);
 }
 
 template <typename T>

@@ -98,6 +98,25 @@ def test_distillation_of_records_that_are_no_numbers(C, planes, S):
     G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), lay_rows(rest, planes), 1.5)
 
 
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("C", [3, 24, 60, 900])
+def test_distillation_of_the_lowest_scores_at_low_temperatures(C, planes, S):
+    """A student's mask of the type's lowest number, on labels that the teacher wants a little, in the record or outside it: a
+    huge loss, but a number, where the score over T is none."""
+    low = torch.finfo(torch.float32).min
+    x = G.scores_of((6, C), torch.float32, 301)
+    values = torch.tensor([[9.0, 4.0], [9.0, -2.0], [0.0, 0.0]] * 2, device="cuda")
+    labels = torch.tensor([[0, 1]] * 6, dtype=torch.int32, device="cuda")
+    rest = torch.tensor([-20.0, -1.0, 0.0] * 2, device="cuda")
+    x[:3, 1] = low
+    x[3:, 2:] = low
+    for t in (0.5, 0.1):
+        for r in (rest, None):
+            G.check_distill(S, lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), t)
+            loss, _ = S.ops.distillation_forward(lay(x, planes), lay(values, planes), lay(labels, planes), None if r is None else lay_rows(r, planes), t)
+            assert torch.isfinite(loss).all() and float(loss.max()) > 1e30
+
+
 @pytest.mark.parametrize("C", [21, 600])
 def test_distillation_temperatures(C, S):
     """T^2 has to be an ordinary fp32 number; at the ends of the range results stay finite."""
