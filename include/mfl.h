@@ -370,7 +370,8 @@ int mfl_top_labels(const void *scores, int dtype, int N, int C, int S, long long
  *   loss = T^2 ( sum_j p_j log(p_j / q_j) + p_rest log(p_rest / q_rest) )
  * Entries with a label outside [0, C) belong to no class and are passed over (a record padded with -1); an entry named
  * twice counts as two entries.  Rows with valid = 0, without any teacher mass or whose scores are all -inf have loss 0
- * and gradient 0, whatever the other tensors hold there.
+ * and gradient 0, whatever the other tensors hold there.  A NaN among a row's scores makes its loss and gradient NaN, one in
+ * its record the loss and the gradients that it enters.
  *   values: [N][k][S] of values_dtype   labels: [N][k][S] int32   rest: [N][S] float or NULL (entries renormalised)
  *   valid: [N][S] bytes or NULL   loss: [N][S]   stats: [5][N][S] floats, from forward to backward (neither written nor
  *   read for C <= MFL_DISTILLATION_LONE_LABELS, where any address but NULL will do)

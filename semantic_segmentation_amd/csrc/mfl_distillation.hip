@@ -20,11 +20,13 @@
 // row with a NaN score: all NaN.  Up to kLoneBlock labels nothing is kept, the backward pass finds them anew.
 //
 // Both passes are bound by memory: the forward pass reads the scores, the backward pass reads them again and writes the
-// gradient.  Measured on MI355X, forward / backward: 8 x 21 x 512 x 512 fp32, k = 4 with rest 58 / 96 us (4.5 TB/s each);
-// 2 x 19 x 1024 x 2048 bf16, k = 3 70 / 112 us (3.6 TB/s: two bytes a lane and the vector unit's share); 2048 x 128000 bf16,
-// k = 64 with rest 99 / 207 us (5.3 / 5.1 TB/s: the backward pass starts with the rows that the forward pass read last, part
-// of which is still in the last-level cache, and streams its gradient past it; rows from the first on 316, cached gradient
-// 377 us for both).  16 x 32000: 20 us of kernels in a call that takes the host 100.
+// gradient.  Measured on MI355X, forward / backward: 8 x 21 x 512 x 512 fp32, k = 4 with rest 64 / 98 us (4.1 / 4.4 TB/s);
+// 2 x 19 x 1024 x 2048 bf16, k = 3 73 / 111 us (3.5 / 3.7 TB/s: two bytes a lane and the vector unit's share); 2048 x 128000
+// bf16, k = 64 with rest 103 / 211 us (5.1 / 5.0 TB/s: the backward pass starts with the rows that the forward pass read last,
+// part of which is still in the last-level cache, and streams its gradient past it; rows from the first on 316, cached gradient
+// 377 us for both).  16 x 32000: 21 us in three launches, of which the bytes take one, in a call that takes the host about 105
+// with autograd's round trip.  Channels-last maps are the lanes' as well, and their stores of single scores C apart, streamed
+// past the caches, do badly: 8 x 21 x 512 x 512 73 / 1459 us in fp32, 55 / 719 in bf16.
 #include "mfl_scores.h"
 
 namespace {
@@ -670,7 +672,9 @@ backward_rows_kernel(Rows in, Teacher t, int parts, const float *__restrict__ st
     }
 }
 
-// (few short rows as well: a lane alone takes its time over a long record)
+// (few short rows as well: a lane alone takes its time over a long record.)  Lanes / rows, fp32, k = 8 with rest, both passes, us:
+// 4096 x 64 37 / 37, 16384 x 64 51 / 85, 16384 x 128 95 / 87, 4096 x 256 103 / 37, 16384 x 512 329 / 97, 131072 x 128 728 / 616.
+// (Many rows of 128 to 511 labels would do better by rows, for the gradient's stores: 131072 x 256 1664 / 616.)
 bool by_rows(const Rows &in) { return in.sc == 1 && (in.C >= 512 || (in.C >= 64 && in.rows <= 16384)); }
 size_t mark_bytes(int C, int parts)
 {

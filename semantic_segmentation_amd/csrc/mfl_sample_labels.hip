@@ -17,12 +17,14 @@
 // Shapes of work: one lane per row (label maps), one wave or workgroup per row where top_k cuts the row to a short list
 // (mfl_wave_top.h), and one workgroup per row otherwise, which finds the cut by a histogram of the weights.
 //
-// Measured on MI355X.  Lanes: 8 x 21 x 512 x 512 fp32 without filters 60 us (3.5 TB/s; a 64-bit exponential is 17
-// instructions, so the vector unit is about as busy as the memory), top_p alone 216; 2 x 150 x 512 x 512 with top_k 5, top_p
-// and min_p 81 us (3.9 TB/s).  Rows: 1 x 128000 bf16, top_k 50, 21 us and 64 x 50001 f16 without filters 20 us (two launches,
-// latency); 256 x 128000 fp32, every row its own temperature and top_p, 133 us: 25 the largest score (the rate of a copy), 40
-// the histogram (64-bit exponentials and LDS atomics), 43 the sweep, the rest scans and the pick; a binary search over whole
-// passes instead of the histogram took 12.9 ms, a fourth pass for the runs 187 us.
+// Measured on MI355X.  Lanes: 8 x 21 x 512 x 512 fp32 without filters 58 us (3.6 TB/s; a 64-bit exponential is 17
+// instructions, so the vector unit is about as busy as the memory), top_p alone 210 (every label is sorted into the list);
+// 2 x 150 x 512 x 512 with top_k 5, top_p and min_p 78 us (4.0 TB/s), top_p alone 1007.  Rows: 1 x 128000 bf16, top_k 50, 21 us
+// and 64 x 50001 f16 without filters 20 us (two launches; the second is 12 us of one workgroup's work); 256 x 128000 fp32, every
+// row its own temperature and top_p, 137 us: 25 the largest score (the rate of a copy), 40 the histogram (64-bit exponentials
+// and LDS atomics), 43 the sweep, the rest scans and the pick; a binary search over whole passes instead of the histogram took
+// 12.9 ms, a fourth pass for the runs 187 us.  Where the cut's bin holds more than its list of 2048, the row is gone over again:
+// 64 x 200000 bf16 at T 1.3 and top_p 0.9 854 us (fp32 153), 4 x 128000 fp32 of standard deviation 0.05 3.5 ms (1: 91 us).
 //
 // A row without a finite largest score (all -inf, or a NaN or +inf among them) has no distribution: label -1, logprob -inf.
 #include "mfl_wave_top.h"
@@ -1678,7 +1680,9 @@ Plan plan_of(const Rows &in, const Settings &set)
         const int parts = row_per_wave(in.rows, in.C) ? 1 : top_parts(in.rows, in.C);
         return parts > 1 ? (size_t)in.rows * parts * part_keys(k) * sizeof(uint64_t) : 0;
     };
-    // lanes: short rows, and planes of many rows
+    // lanes: short rows, and planes of many rows.  Lanes / rows of neighbouring labels, fp32, without filters, top_k 8 and top_p,
+    // us: 4096 x 64 19 / 40, 14 / 15, 52 / 73; 4096 x 256 42 / 35, 35 / 22, 309 / 72; 16384 x 256 42 / 123, 34 / 64, 310 / 255.
+    // (Many rows of 256 and more labels would do better with lanes: 131072 x 256 83 / 959, 79 / 421, 487 / 1991.)
     if (!(in.sc == 1 && in.C >= 256) && !(in.C >= 1024 && in.rows <= 4096)) {
         const int list = k ? k : no_k && in.C <= 32 ? in.C : 0;
         if (plain) return {in.C <= kLoneBlock ? LONE : LANES, 0, false, false, 0};

@@ -6,15 +6,17 @@
 //
 // Two shapes of work, here and in the other operators on rows.
 //   lanes   one lane per row, the k best in the lane's registers, labels streamed once.  Neighbouring pixels of a label
-//           map are neighbouring lanes, so every load of a class plane is coalesced.  A new score is sorted in; what falls
-//           off the list's end can no longer be among the k best and goes into the rest's running sum, so one pass gives
-//           both and the rest is never a difference of two sums.
+//           map are neighbouring lanes, so every load of a class plane is coalesced (where few labels lie side by side, in
+//           channels-last maps and matrices, lanes are C scores apart and a line is read in C loads).  A new score is sorted
+//           in; what falls off the list's end can no longer be among the k best and goes into the rest's running sum, so one
+//           pass gives both and the rest is never a difference of two sums.
 //   rows    one or more waves per row, for rows of many labels (mfl_wave_top.h).
 //
-// Measured on MI355X.  Lanes, 8 x 21 x 512 x 512 fp32, k = 4: 51 us, 4.9 TB/s, the rate of a large copy; 4 x 150 x 512 x 512,
-// k = 8: 164 us, 4.3 TB/s (the list as separate words for score and label: 198 us, bound by the vector unit).  Rows,
-// 1024 x 32001 bf16, k = 64: 36 us, 1.8 TB/s, bound by the vector unit (about 20 instructions a score, 9 of them the rest's
-// exponential and sum).
+// Measured on MI355X.  Lanes, 8 x 21 x 512 x 512 fp32, k = 4: 51 us, 4.9 TB/s, the rate of a large copy (channels-last 114 us;
+// bf16 44 and 59); 4 x 150 x 512 x 512, k = 8: 161 us, 4.3 TB/s (the list as separate words for score and label: 198 us, bound
+// by the vector unit).  Rows, 1024 x 32001 bf16, k = 64: 36 us, 1.8 TB/s, bound by the vector unit (about 20 instructions a
+// score, 9 of them the rest's exponential and sum); where a mask leaves ten labels of each row 81 us, since every -inf then
+// reaches the list's bound.  Maps with k > 32, a wave a pixel: 2 x 150 x 512 x 512, k = 40, 1017 us.
 #include "mfl_wave_top.h"
 
 namespace {
@@ -145,7 +147,9 @@ top_join_kernel(Rows in, float c2, float inv_t, int k, int parts, const uint64_t
     put_row(top, in, r, k, inv_t, values, labels, rest);
 }
 
-// Rows of many neighbouring labels, long lists, and few rows go to waves
+// Rows of many neighbouring labels, long lists, and few rows go to waves.  Lanes / waves, fp32, k = 4, us: 4096 x 64 14 / 13,
+// 16384 x 64 13 / 23, 4096 x 256 32 / 14, 16384 x 256 32 / 37, 16384 x 512 60 / 38, 131072 x 1024 356 / 335.  (Many rows of
+// 256 to 1000 labels would do better with lanes: 131072 x 256 80 / 236.)
 bool by_waves(const Rows &in, int k)
 {
     return k > 32 || in.C > kBestLabels || (in.sc == 1 && (in.C >= 256 || (in.C >= 64 && in.rows <= 4096))) || (in.C >= 1024 && in.rows <= 4096);
