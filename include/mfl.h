@@ -352,8 +352,8 @@ int mfl_resize_labels(const unsigned char *src, int H0, int W0, const int *yin, 
  * Results do not depend on the launch or on timing: no floating-point atomics.
  *
  * mfl_top_labels: the k largest scores of every row, descending, the lower label first among equals (a NaN counts as
- * larger than any number), and rest = log sum exp(b) over the other labels (-inf if there are none): what a teacher
- * keeps for mfl_distillation_*.  k = 1 answers like mfl_argmax_labels.  The reference has no counterpart.
+ * larger than any number), and rest = log sum exp(b) over the other labels (-inf if there are none, NaN with a NaN among
+ * them): what a teacher keeps for mfl_distillation_*.  k = 1 answers like mfl_argmax_labels.  The reference has no counterpart.
  *   values: [N][k][S] of the scores' type   labels: [N][k][S] int32   rest: [N][S] float
  *   1 <= k <= min(C, MFL_MAX_TOP_LABELS), 1e-30 <= temperature <= 1e30
  */

@@ -69,11 +69,12 @@ __device__ inline Target target_of(const Teacher &t, Excess sum, bool named, flo
 }
 __device__ inline float log_share(const Teacher &t, const Target &g, float value) { return (value - g.m) * t.inv_t - g.l; }
 
-// p T d; nothing where p is 0.  (A share that fp32 does not hold still counts next to a difference near the largest number.)
+// p T d; nothing where p is 0.  (A share that fp32 does not hold still counts next to a difference near the largest number, but
+// not next to an infinite one.)
 __device__ inline float share_term(float log_p, float t, float d)
 {
     const float e = log_p * kLog2e;
-    const bool tiny = e < -100.f;
+    const bool tiny = e < -100.f && fabsf(d) < INFINITY;
     const float p = __builtin_amdgcn_exp2f(tiny ? e + 60.f : e);
     return p == 0.f ? 0.f : p * t * (tiny ? d * 0x1p-60f : d);
 }

@@ -118,6 +118,18 @@ def test_distillation_of_the_lowest_scores_at_low_temperatures(C, planes, S):
 
 
 @pytest.mark.parametrize("C", [21, 600])
+def test_distillation_of_forbidden_labels_that_the_teacher_hardly_wants(C, S):
+    """A share below 2^-126 is 0 next to a student's -inf, a larger one makes the loss infinite; the gradients are finite."""
+    x = torch.zeros(2, C, device="cuda")
+    x[:, 1] = -INF
+    values = torch.tensor([[0.0, -100.0], [0.0, -70.0]], device="cuda")
+    labels = torch.tensor([[0, 1]] * 2, dtype=torch.int32, device="cuda")
+    loss, stats = S.ops.distillation_forward(x, values, labels)
+    assert abs(float(loss[0]) - np.log(C - 1.0)) <= (G.CHAIN(C) * 2.0 ** -23 + 2.0 ** -21) * (1 + 2 * np.log(C)) and float(loss[1]) == INF
+    assert torch.isfinite(S.ops.distillation_backward(x, values, labels, stats, torch.ones_like(loss))).all()
+
+
+@pytest.mark.parametrize("C", [21, 600])
 def test_distillation_temperatures(C, S):
     """T^2 has to be an ordinary fp32 number; at the ends of the range results stay finite."""
     x = G.scores_of((3, C), torch.float32, 231)
